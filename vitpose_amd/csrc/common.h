@@ -138,8 +138,8 @@ __device__ __forceinline__ void lds_fence(bf16x8 (&f)[N_][S_]) {
 // bf16 resolution of the values they are stored as, and below what the bf16 rounding of the pre-activation itself
 // does to them; degree 15 on [0, 5] reaches 2e-6 / 8e-6 for four more FMAs per value, which showed as 1-2 us per
 // K = 768 launch: the arithmetic of these epilogues is 7-10 us of a 75-110 us launch, measured by removing it).
-// 13 full-rate FMAs per value, packed two per instruction.  NaN propagates through gelu (x enters the result arithmetically).
-// (four values at a time: the two packed FMAs of a Horner step are independent, so the dependent chain of one never
+// 13 full-rate FMAs per value.  NaN propagates through gelu (x enters the result arithmetically).
+// (four values at a time: the FMAs of a Horner step are independent, so the dependent chain of one never
 // waits on itself)
 template <int NC>
 __device__ __forceinline__ f32x4 gelu_poly(f32x4 s, const float (&c)[NC]) {
