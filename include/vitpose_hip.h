@@ -493,6 +493,25 @@ int vp_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, co
                   const int* chunk_len, const float* chunk_lr_scale, const float* chunk_wd, int nchunks,
                   float lr, float beta1, float beta2, float eps, int step, const float* gnorm_sq,
                   float max_norm, float grad_scale, vp_stream_t stream);
+/* The same step with both moments in 8 bits.  The state of element i of a chunk lives at chunk_state[c] + i of two e4m3
+ * (OCP, finite) arrays of state_numel values (a multiple of 128), with one f32 scale per 128 of them:
+ *   exp_avg = m_e4m3 * m_scale (rounded to nearest),  sqrt(exp_avg_sq) = r_e4m3 * r_scale (rounded to one of the two
+ * neighbours, up with the probability that keeps the expected exp_avg_sq; never from non-zero to zero).  `noise` keys the
+ * random numbers (a hash of the low 32 bits of the state position and the key): another one each step, the same on every
+ * replica.  A block whose largest magnitude is under 2^-100 is stored as zeros; one that holds anything not finite gets a
+ * NaN scale.  Table: chunk_len in 1..2048 and chunk_start multiples of 4, chunk_state multiples of 128, no two chunks
+ * overlapping; a row that breaks this or leaves the buffers (numel = floats of p) is skipped.
+ * norm_partials (npartials <= 256 doubles of vp_sumsq_chunks_f64, or NULL and 0): gradients are multiplied by grad_scale *
+ * min(1, max_norm / (norm * grad_scale + 1e-6)). */
+int vp_adamw8_step(float* p, const float* g, void* m_e4m3, float* m_scale, void* r_e4m3, float* r_scale, void* p_bf16,
+                   const long* chunk_start, const int* chunk_len, const float* chunk_lr_scale, const float* chunk_wd,
+                   const long* chunk_state, int nchunks, long numel, long state_numel, double lr, double beta1,
+                   double beta2, double eps, long step, const double* norm_partials, int npartials, float max_norm,
+                   float grad_scale, unsigned noise, vp_stream_t stream);
+/* partials[0 .. npartials) = partial sums of x^2 over the table's chunks in 64 bits, in an order that depends on the table
+ * and on npartials alone (1..256 workgroups; the caller's next launch adds them up). */
+int vp_sumsq_chunks_f64(const float* x, const long* chunk_start, const int* chunk_len, int nchunks, long numel,
+                        double* partials, int npartials, vp_stream_t stream);
 
 #ifdef __cplusplus
 }

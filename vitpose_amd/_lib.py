@@ -7,7 +7,7 @@ import ctypes
 import os
 
 import torch  # noqa: F401  (first: the library must bind to the HIP runtime torch has loaded)
-from ctypes import POINTER, Structure, c_float, c_int, c_long, c_size_t, c_void_p
+from ctypes import POINTER, Structure, c_double, c_float, c_int, c_long, c_size_t, c_uint, c_void_p
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 ABI_VERSION = 4   # VP_ABI_VERSION of include/vitpose_hip.h this binding was written for
@@ -122,6 +122,9 @@ SIGNATURES = {
     'vp_pos_embed_grad': [P, P, c_int, c_int, c_int, P],
     'vp_adamw_step': [P, P, P, P, P, P, P, P, P, c_int, c_float, c_float, c_float, c_float, c_int, P,
                       c_float, c_float, P],
+    'vp_sumsq_chunks_f64': [P, P, P, c_int, c_long, P, c_int, P],
+    'vp_adamw8_step': [P] * 12 + [c_int, c_long, c_long, c_double, c_double, c_double, c_double, c_long, P, c_int,
+                                  c_float, c_float, c_uint, P],
 }
 
 _lib = None
@@ -147,6 +150,20 @@ def lib():
         fn.restype = c_int
     _lib = L
     return L
+
+
+def launch(device, name, *args):
+    """Call one entry point on `device` (made current for the call if it is not) and on its current stream; pointers
+    are plain integers.  A non-zero status raises."""
+    fn = getattr(lib(), name)
+    index = device.index
+    if index is None or index == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        raise RuntimeError(f'{name} failed: {rc}')
 
 
 def exported_symbols():

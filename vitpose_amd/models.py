@@ -1305,7 +1305,8 @@ class TopDown(nn.Module):
     def build_optimizer(self, optimizer_cfg: dict, grad_clip: Optional[dict] = None):
         """Fused layer-decay AdamW over the flat store from the reference's `optimizer=dict(type='AdamW',
         ..., constructor='LayerDecayOptimizerConstructor', paramwise_cfg=dict(num_layers, layer_decay_rate))`
-        and `optimizer_config=dict(grad_clip=dict(max_norm, norm_type=2))` blocks."""
+        and `optimizer_config=dict(grad_clip=dict(max_norm, norm_type=2))` blocks.  Extension: `state_bits=8` in the
+        optimizer block holds both moments in 8 bits (`noise_seed` keys their rounding)."""
         if self._engine is None:
             raise RuntimeError('build_optimizer needs the fused model on a HIP device (model.cuda())')
         cfg = dict(optimizer_cfg)
@@ -1319,7 +1320,8 @@ class TopDown(nn.Module):
                                      weight_decay=cfg.get('weight_decay', 1e-2),
                                      layer_decay_rate=pw.get('layer_decay_rate', 1.0),
                                      num_layers=pw.get('num_layers', self.backbone.depth),
-                                     max_grad_norm=(grad_clip or {}).get('max_norm', 0.0), frozen=frozen)
+                                     max_grad_norm=(grad_clip or {}).get('max_norm', 0.0), frozen=frozen,
+                                     state_bits=cfg.get('state_bits', 32), noise_seed=cfg.get('noise_seed', 0))
         return _FlatOptimizer(self)
 
     def enable_ddp(self, process_group=None, blocks_per_bucket=4):

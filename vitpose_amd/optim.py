@@ -4,9 +4,12 @@ reference's LayerDecayOptimizerConstructor
 schedule of the ViTPose configs, and the chunk table that drives the fused AdamW
 kernel over the flat parameter buffer.
 """
+from ctypes import c_void_p
 from typing import Dict, List, Sequence, Tuple
 
 import torch
+
+from . import _lib
 
 CHUNK = 1 << 11  # elements per AdamW workgroup: two float4 per lane; measured 596 us per step for 90 M
 # parameters (norm + update) against 637 us at 1 << 16, whose 1472 workgroups leave an uneven last round
@@ -51,17 +54,119 @@ def step_lr(base_lr: float, it: int, epoch: int, steps=(170, 200), gamma=0.1, wa
     return lr
 
 
+# ---------------------------------------------------------------------------------------------------------------
+# moments in 8 bits
+# ---------------------------------------------------------------------------------------------------------------
+STATE_BLOCK = 128      # state values that share one scale
+_F8 = torch.float8_e4m3fn
+
+
+def new_state8(numel: int, device):
+    """Zero moments for `numel` state values (a multiple of 128): (exp_avg e4m3 [numel], its scales f32 [numel / 128],
+    sqrt(exp_avg_sq) e4m3 [numel], its scales f32 [numel / 128])."""
+    if numel % STATE_BLOCK:
+        raise ValueError(f'state values come in blocks of {STATE_BLOCK}, got {numel}')
+
+    def codes():
+        return torch.zeros(numel, dtype=torch.uint8, device=device).view(_F8)
+
+    def scales():
+        return torch.zeros(numel // STATE_BLOCK, dtype=torch.float32, device=device)
+    return codes(), scales(), codes(), scales()
+
+
+def noise_key(seed: int, step: int) -> int:
+    """The `noise` argument of step number `step` of a run with `seed`: 31 bits, the same on every rank."""
+    def mix(h):
+        h ^= h >> 16
+        h = h * 0x85EBCA6B & 0xFFFFFFFF
+        h ^= h >> 13
+        h = h * 0xC2B2AE35 & 0xFFFFFFFF
+        return h ^ (h >> 16)
+    return mix((seed & 0xFFFFFFFF) ^ mix(step & 0xFFFFFFFF)) & 0x7FFFFFFF
+
+
+def _flat_arg(t, dtype, name, device, numel=None):
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype:
+        raise TypeError(f'{name}: expected a {dtype} tensor, got {getattr(t, "dtype", type(t).__name__)}')
+    if t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f'{name}: must be one-dimensional and contiguous')
+    if t.device != device:
+        raise ValueError(f'{name}: on {t.device}, the parameters on {device}')
+    if numel is not None and t.numel() != numel:
+        raise ValueError(f'{name}: {t.numel()} values, expected {numel}')
+
+
+def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8, step, noise, half=None,
+                max_grad_norm=0.0, grad_scale=1.0):
+    """One AdamW step over flat f32 buffers whose moments are held in 8 bits (torch.optim.AdamW's update).
+
+    param, grad: f32 [numel];  half: bf16 [numel] copy of the new weights, or None;  state: as `new_state8` makes it;
+    chunks: device tensors (start int64, length int32, lr_scale f32, weight_decay f32, state_start int64), one entry per
+    run of at most 2048 consecutive elements of one tensor (starts and lengths multiples of 4, state starts multiples
+    of 128, no overlaps; an entry that leaves the buffers is skipped);  step: number of this step, from 1;  noise: key
+    of this step's random numbers (`noise_key`).  max_grad_norm > 0 clips the gradients of the table's elements by their
+    norm first.  Everything is updated in place on the current stream; nothing synchronises."""
+    dev = param.device
+    if dev.type != 'cuda':
+        raise RuntimeError('adamw8_step runs on a HIP device only')
+    n = param.numel()
+    _flat_arg(param, torch.float32, 'param', dev)
+    _flat_arg(grad, torch.float32, 'grad', dev, n)
+    if half is not None:
+        _flat_arg(half, torch.bfloat16, 'half', dev, n)
+    m8, ms, r8, rs = state
+    ns = m8.numel()
+    if ns % STATE_BLOCK:
+        raise ValueError(f'state values come in blocks of {STATE_BLOCK}, got {ns}')
+    _flat_arg(m8, _F8, 'exp_avg', dev)
+    _flat_arg(r8, _F8, 'exp_avg_sq', dev, ns)
+    _flat_arg(ms, torch.float32, 'exp_avg scale', dev, ns // STATE_BLOCK)
+    _flat_arg(rs, torch.float32, 'exp_avg_sq scale', dev, ns // STATE_BLOCK)
+    start, length, lr_scale, decay, state_start = chunks
+    nc = start.numel()
+    _flat_arg(start, torch.int64, 'chunk start', dev)
+    _flat_arg(length, torch.int32, 'chunk length', dev, nc)
+    _flat_arg(lr_scale, torch.float32, 'chunk lr scale', dev, nc)
+    _flat_arg(decay, torch.float32, 'chunk weight decay', dev, nc)
+    _flat_arg(state_start, torch.int64, 'chunk state start', dev, nc)
+    b1, b2 = betas
+    if step < 1 or not (0 <= b1 < 1 and 0 <= b2 < 1) or eps < 0:
+        raise ValueError(f'step {step}, betas {betas}, eps {eps}: step >= 1, betas in [0, 1) and eps >= 0 needed')
+    if not 0 <= noise < 1 << 32:
+        raise ValueError('noise is a 32-bit key')
+    if nc == 0:
+        return
+    partials, npart = None, 0
+    if max_grad_norm > 0:
+        npart = min(256, (nc + 3) // 4)
+        partials = torch.empty(npart, dtype=torch.float64, device=dev)
+        _lib.launch(dev, 'vp_sumsq_chunks_f64', grad.data_ptr(), start.data_ptr(), length.data_ptr(), nc, n,
+                    partials.data_ptr(), npart)
+    _lib.launch(dev, 'vp_adamw8_step', param.data_ptr(), grad.data_ptr(), m8.data_ptr(), ms.data_ptr(), r8.data_ptr(),
+                rs.data_ptr(), half.data_ptr() if half is not None else None, start.data_ptr(), length.data_ptr(),
+                lr_scale.data_ptr(), decay.data_ptr(), state_start.data_ptr(), nc, n, ns, lr, b1, b2, eps, step,
+                partials.data_ptr() if npart else None, npart, max_grad_norm, grad_scale, noise)
+
+
 class FlatAdamW:
-    """torch.optim.AdamW semantics over a ParamStore, one fused kernel per step."""
+    """torch.optim.AdamW semantics over a ParamStore, one fused kernel per step.
+
+    state_bits = 8 holds both moments in 8 bits (`adamw8_step`; 2.06 bytes of state a parameter instead of 8): its
+    random numbers follow from `noise_seed` and the step count, so ranks that hold the same gradients stay identical."""
 
     def __init__(self, store, groups: Dict[str, dict], lr: float, betas=(0.9, 0.999), eps=1e-8,
-                 max_grad_norm: float = 0.0, frozen: Sequence[str] = ()):
+                 max_grad_norm: float = 0.0, frozen: Sequence[str] = (), state_bits: int = 32, noise_seed: int = 0):
+        if state_bits not in (8, 32):
+            raise ValueError(f'state_bits is 8 or 32, got {state_bits}')
+        self.state_bits, self.noise_seed = state_bits, noise_seed
         self.store, self.lr, self.betas, self.eps = store, lr, betas, eps
         self.max_grad_norm = max_grad_norm
         self.step_count = 0
         self.frozen = tuple(frozen)
         dev = store.device
-        starts, lens, scales, wds = [], [], [], []
+        starts, lens, scales, wds, sstarts, soff = [], [], [], [], [], 0
+        self.state_offsets = {}
         for name in store.names:
             if name in frozen:
                 continue
@@ -69,16 +174,23 @@ class FlatAdamW:
             n = store.view(name).numel()
             n_pad = (n + 3) // 4 * 4  # padding inside the 64-element alignment gap: zeros stay zeros
             off = store.offsets[name]
+            self.state_offsets[name] = soff
             for c0 in range(0, n_pad, CHUNK):
                 starts.append(off + c0)
                 lens.append(min(CHUNK, n_pad - c0))
                 scales.append(grp['lr_scale'])
                 wds.append(grp['weight_decay'])
+                sstarts.append(soff + c0)
+            soff += (n_pad + STATE_BLOCK - 1) // STATE_BLOCK * STATE_BLOCK
         self.nchunks = len(starts)
         self.chunk_start = torch.tensor(starts, dtype=torch.int64, device=dev)
         self.chunk_len = torch.tensor(lens, dtype=torch.int32, device=dev)
         self.chunk_lr_scale = torch.tensor(scales, dtype=torch.float32, device=dev)
         self.chunk_wd = torch.tensor(wds, dtype=torch.float32, device=dev)
+        if state_bits == 8:
+            self.chunk_state = torch.tensor(sstarts, dtype=torch.int64, device=dev)
+            self.state8 = new_state8(soff, dev)
+            return
         self.exp_avg = torch.zeros_like(store.data)
         self.exp_avg_sq = torch.zeros_like(store.data)
         self.gnorm_sq = torch.zeros(1, dtype=torch.float32, device=dev)
@@ -87,8 +199,15 @@ class FlatAdamW:
         self.gnorm_partials = torch.zeros(2048, dtype=torch.float32, device=dev)
 
     def step(self, lr: float = None, grad_scale: float = 1.0):
-        from . import _lib
-        from ctypes import c_void_p
+        if self.state_bits == 8:
+            st = self.store
+            self.step_count += 1
+            adamw8_step(st.data, st.grad, self.state8, (self.chunk_start, self.chunk_len, self.chunk_lr_scale,
+                                                        self.chunk_wd, self.chunk_state),
+                        lr=self.lr if lr is None else lr, betas=self.betas, eps=self.eps, step=self.step_count,
+                        noise=noise_key(self.noise_seed, self.step_count), half=st.half,
+                        max_grad_norm=self.max_grad_norm, grad_scale=grad_scale)
+            return
         L = _lib.lib()
         s = c_void_p(torch.cuda.current_stream().cuda_stream)
         st = self.store
@@ -117,24 +236,49 @@ class FlatAdamW:
     # -- checkpointing (the reference saves optimizer.state_dict() next to the weights,
     #    mmcv_custom/checkpoint.py:490-552; runner.resume restores it) --
     def state_dict(self):
-        """Adam moments per parameter NAME (CPU tensors) + the step count and hyper-parameters."""
+        """Adam moments per parameter NAME (CPU tensors) + the step count and hyper-parameters.  8-bit moments are
+        saved as they are held (e4m3 codes as bytes + block scales), so that a resumed run continues bit for bit."""
         st = self.store
         names = [n for n in st.names if n not in self.frozen]
+        if self.state_bits == 8:
+            return {'format': 'vitpose_amd.FlatAdamW8/1', 'step': self.step_count, 'noise_seed': self.noise_seed,
+                    'hyper': dict(lr=self.lr, betas=tuple(self.betas), eps=self.eps, max_grad_norm=self.max_grad_norm),
+                    'state': {n: {k: v.detach().cpu().clone() for k, v in self._state8_views(n).items()} for n in names}}
         return {'format': 'vitpose_amd.FlatAdamW/1', 'step': self.step_count,
                 'hyper': dict(lr=self.lr, betas=tuple(self.betas), eps=self.eps, max_grad_norm=self.max_grad_norm),
                 'state': {n: {'exp_avg': st._v(self.exp_avg, n).detach().cpu().clone(),
                               'exp_avg_sq': st._v(self.exp_avg_sq, n).detach().cpu().clone()} for n in names}}
 
+    def _state8_views(self, name):
+        """The blocks of one parameter in the 8-bit state, codes as bytes."""
+        n = self.store.view(name).numel()
+        b0 = self.state_offsets[name] // STATE_BLOCK
+        b1 = b0 + (n + STATE_BLOCK - 1) // STATE_BLOCK
+        m8, ms, r8, rs = self.state8
+        return {'exp_avg': m8.view(torch.uint8)[b0 * STATE_BLOCK:b1 * STATE_BLOCK], 'exp_avg_scale': ms[b0:b1],
+                'exp_avg_sq_root': r8.view(torch.uint8)[b0 * STATE_BLOCK:b1 * STATE_BLOCK], 'exp_avg_sq_scale': rs[b0:b1]}
+
     def load_state_dict(self, sd):
-        if sd.get('format') != 'vitpose_amd.FlatAdamW/1':
-            raise ValueError('not a FlatAdamW state dict (expected format "vitpose_amd.FlatAdamW/1")')
+        want = 'vitpose_amd.FlatAdamW8/1' if self.state_bits == 8 else 'vitpose_amd.FlatAdamW/1'
+        if sd.get('format') != want:
+            raise ValueError(f'not a FlatAdamW state dict of {self.state_bits}-bit moments (expected format "{want}")')
         st = self.store
         names = [n for n in st.names if n not in self.frozen]
         missing = [n for n in names if n not in sd['state']]
         unexpected = [n for n in sd['state'] if n not in names]
         if missing or unexpected:
             raise KeyError(f'optimizer state does not match the model: missing {missing[:3]}, unexpected {unexpected[:3]}')
-        for n in names:
+        if self.state_bits == 8:
+            for n in names:
+                for key, view in self._state8_views(n).items():
+                    v = sd['state'][n][key]
+                    if v.shape != view.shape or v.dtype != view.dtype:
+                        raise ValueError(f'{n}.{key}: {v.dtype} {tuple(v.shape)} != {view.dtype} {tuple(view.shape)}')
+            for n in names:
+                for key, view in self._state8_views(n).items():
+                    view.copy_(sd['state'][n][key])
+            self.noise_seed = int(sd['noise_seed'])
+        for n in names if self.state_bits == 32 else ():
             for key, buf in (('exp_avg', self.exp_avg), ('exp_avg_sq', self.exp_avg_sq)):
                 v = sd['state'][n][key]
                 if tuple(v.shape) != tuple(st.shapes[n]):
