@@ -345,6 +345,40 @@ int vp_wgrad_grouped_bf16(const vp_group_entry* table_dev, int count, int total_
 int vp_wgrad_grouped_kmap_bf16(const vp_group_entry* table_dev, int count, int total_tiles, int K,
                                vp_stream_t stream);
 
+/* ------------------------------------------------------------- Expert layers ------
+ * A Linear whose weight depends on the row (MoEMlp.experts, mmpose/models/backbones/vit_moe.py:92-111, where the choice is
+ * per image): rows grouped by expert, any number of rows per expert, none included.
+ *   vp_expert_rows: expert [T] int32 -> rows [T] = the row numbers in the order of their experts (rows of one expert in
+ *     ascending order; rows whose entry is not in [0, E) come last), offsets [E + 1] = where each expert's rows begin, and
+ *     where the last one's end.  E <= 512 (VP_ERR_UNSUPPORTED beyond).
+ *   The products take such a list, or rows = NULL: entry i of the list is then row i.  Entries outside [0, T) are left
+ *     out, offsets are cut to [0, T]; no row may be listed twice.  bf16 operands, sums in f32, each result rounded once.
+ *     x [T][ldx >= K], w [E][N][ldw >= K] (experts stride_w apart), dy [T][ldy >= N], bias [E][N] f32 (stride_b apart).
+ *     N, K and every leading dimension multiples of 8, pointers on 16 bytes.
+ *     fwd:   out [T][ldo >= N] bf16 = x w^T + bias
+ *     dgrad: out [T][ldo >= K] bf16 = dy w
+ *     wgrad: dw [E][N][K] f32 = dy^T x, db [E][N] f32 (optional) = column sums of dy; zeros for an expert without rows.
+ *            The rows are cut into s = vp_grouped_wgrad_slices(T, E, N, K) slices where there are few tiles; s > 1 needs a
+ *            workspace of s E N (K + (db ? 1 : 0)) floats.  Partial sums are added up in a fixed order.
+ *     zero_rest: fwd / dgrad write zeros into the rows that no expert takes (list entries behind offsets[E]); otherwise
+ *     those rows are left as they are. */
+typedef struct vp_grouped_args {
+    int T, E, N, K;
+    const int* offsets; const int* rows;
+    const void* x; long ldx;
+    const void* w; long ldw, stride_w;
+    const float* bias; long stride_b;
+    const void* dy; long ldy;
+    void* out; long ldo;
+    int zero_rest;
+} vp_grouped_args;
+int vp_expert_rows(const int* expert, int T, int E, int* rows, int* offsets, vp_stream_t stream);
+int vp_grouped_fwd(const vp_grouped_args* args, vp_stream_t stream);
+int vp_grouped_dgrad(const vp_grouped_args* args, vp_stream_t stream);
+int vp_grouped_wgrad(const vp_grouped_args* args, float* dw, float* db, void* workspace, size_t workspace_bytes,
+                     vp_stream_t stream);
+int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: no stream argument */
+
 /* --------------------------------------------------------------- Input side ------
  * vp_warp_affine_normalize: TopDownAffine's cv2.warpAffine(img, trans, image_size, INTER_LINEAR)
  *   (datasets/pipelines/top_down_transform.py:312-363) + ToTensor + NormalizeTensor (shared_transform.py:21-64)

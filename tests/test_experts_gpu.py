@@ -1,0 +1,328 @@
+"""Expert products (vp_expert_rows, vp_grouped_*, vitpose_amd.experts) against sums in 64 bits.
+
+Tolerances: a sum of n products in f32 is off by at most (n + 2) 2^-24 of the sum of their magnitudes, in any order; a bf16
+result by half a step more, 2^-8 of itself.  Products of small whole numbers whose sums stay below 2^8 are exact in both."""
+import pytest
+import torch
+
+from vitpose_amd import experts
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def routing(T, E, kind, seed):
+    g = torch.Generator().manual_seed(seed)
+    if kind == 'even':
+        ids = torch.arange(T) % E
+    elif kind == 'one':
+        ids = torch.full((T,), E - 1)
+    elif kind == 'gaps':              # every other expert without a row, some rows without an expert
+        ids = torch.randint(0, E, (T,), generator=g) // 2 * 2
+        ids[torch.rand(T, generator=g) < 0.1] = -1
+        ids[torch.rand(T, generator=g) < 0.05] = E + 3
+    else:                             # most rows at the first experts
+        ids = (torch.rand(T, generator=g) ** 4 * E).long().clamp(max=E - 1)
+    return ids[torch.randperm(T, generator=g)].int()
+
+
+def lists(ids, E):
+    key = torch.where((ids >= 0) & (ids < E), ids, torch.full_like(ids, E))
+    order = torch.sort(key, stable=True).indices.int()
+    count = torch.bincount(key.long(), minlength=E + 1)[:E]
+    return order, torch.cat([torch.zeros(1, dtype=torch.long), count.cumsum(0)]).int()
+
+
+def oracle(x, w, b, dy, ids):
+    """(y, dx, dw, db) in 64 bits and the sums of magnitudes behind them."""
+    x, w, dy = x.double(), w.double(), dy.double()
+    E = w.shape[0]
+    y, ya = torch.zeros(2, x.shape[0], w.shape[1], dtype=torch.float64)
+    dx, dxa = torch.zeros(2, *x.shape, dtype=torch.float64)
+    dw, dwa = torch.zeros(2, *w.shape, dtype=torch.float64)
+    db, dba = torch.zeros(2, E, w.shape[1], dtype=torch.float64)
+    for e in range(E):
+        m = (ids == e).nonzero().flatten()
+        if m.numel():
+            y[m], ya[m] = x[m] @ w[e].t(), x[m].abs() @ w[e].abs().t()
+            if b is not None:
+                y[m] += b[e].double()
+                ya[m] += b[e].double().abs()
+            dx[m], dxa[m] = dy[m] @ w[e], dy[m].abs() @ w[e].abs()
+            dw[e], dwa[e] = dy[m].t() @ x[m], dy[m].abs().t() @ x[m].abs()
+            db[e], dba[e] = dy[m].sum(0), dy[m].abs().sum(0)
+    return (y, dx, dw, db), (ya, dxa, dwa, dba)
+
+
+def close(got, want, mags, n, what):
+    tol = (n + 2) * U * mags + (2.0 ** -8 * want.abs() if got.dtype == torch.bfloat16 else 0)
+    off = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all(), what
+    assert (off <= tol).all(), f'{what}: worst {((off - tol) / (tol + 1e-300)).max().item():.3g} over the bound at {(off - tol).argmax().item()}'
+
+
+CASES = [
+    # T, E, K, N, routing
+    (1, 1, 8, 8, 'even'), (1, 6, 1536, 96, 'one'), (2, 5, 64, 16, 'even'), (7, 3, 72, 24, 'gaps'), (64, 4, 128, 64, 'even'),
+    (65, 2, 136, 72, 'one'), (128, 1, 64, 128, 'even'), (129, 8, 200, 136, 'skewed'), (192, 6, 1024, 256, 'gaps'),
+    (300, 64, 96, 40, 'even'), (333, 100, 64, 64, 'skewed'), (600, 512, 40, 24, 'even'), (1000, 6, 1280, 320, 'skewed'),
+    (1537, 3, 264, 200, 'gaps'), (2048, 1, 72, 8, 'even'), (5003, 24, 88, 104, 'gaps'), (9000, 2, 64, 64, 'skewed'),
+    (40000, 7, 16, 8, 'gaps'),
+]
+
+
+def data(T, E, K, N, seed, whole=False):
+    g = torch.Generator().manual_seed(seed)
+
+    def rnd(*s):
+        if whole:
+            return torch.randint(-1, 2, s, generator=g).bfloat16()
+        return (torch.randn(*s, generator=g) * torch.exp(torch.randn(s[-1], generator=g))).bfloat16()
+    return rnd(T, K), rnd(E, N, K), torch.randn(E, N, generator=g), rnd(T, N)
+
+
+@pytest.mark.parametrize('T,E,K,N,kind', CASES)
+def test_rows_are_ordered_by_expert(T, E, K, N, kind):
+    ids = routing(T, E, kind, T)
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    order, offs = lists(ids, E)
+    assert torch.equal(offsets.cpu(), offs) and torch.equal(rows.cpu(), order)
+
+
+def test_rows_of_none_and_of_one():
+    rows, offsets = experts.expert_rows(torch.empty(0, dtype=torch.int32, device='cuda'), 3)
+    assert rows.numel() == 0 and offsets.tolist() == [0, 0, 0, 0]
+    rows, offsets = experts.expert_rows(torch.tensor([-7], dtype=torch.int32, device='cuda'), 2)
+    assert rows.tolist() == [0] and offsets.tolist() == [0, 0, 0]
+
+
+@pytest.mark.parametrize('T,E,K,N,kind', CASES)
+@pytest.mark.parametrize('listed', [True, False])
+def test_products_match_sums_in_64_bits(T, E, K, N, kind, listed):
+    ids = routing(T, E, kind, T + 1)
+    x, w, b, dy = data(T, E, K, N, T + 2)
+    order, offsets = lists(ids, E)
+    if not listed:                    # the arrays lie in the order of the experts; rows of no expert last
+        ids = ids[order.long()]
+        rows = None
+    else:
+        rows = order.cuda()
+    offsets = offsets.cuda()
+    (y, dx, dw, db), (ya, dxa, dwa, dba) = oracle(x, w, b, dy, ids)
+    xd, wd, bd, dyd = x.cuda(), w.cuda(), b.cuda(), dy.cuda()
+    got_dw, got_db = experts.grouped_linear_wgrad(dyd, xd, offsets, rows)
+    n = int(torch.bincount(ids[(ids >= 0) & (ids < E)].long(), minlength=E).max())
+    close(experts.grouped_linear(xd, wd, bd, offsets, rows), y, ya, K + 1, 'y')
+    close(experts.grouped_linear(xd, wd, None, offsets, rows), oracle(x, w, None, dy, ids)[0][0], ya, K, 'y without bias')
+    close(experts.grouped_linear_dgrad(dyd, wd, offsets, rows), dx, dxa, N, 'dx')
+    close(got_dw, dw, dwa, n, 'dw')
+    close(got_db, db, dba, n, 'db')
+    again = experts.grouped_linear_wgrad(dyd, xd, offsets, rows)
+    assert torch.equal(again[0], got_dw) and torch.equal(again[1], got_db)
+
+
+@pytest.mark.parametrize('T,E,K,N,kind', [c for c in CASES if c[2] <= 256 and c[3] <= 256])
+def test_whole_numbers_come_out_exactly(T, E, K, N, kind):
+    """Also the test against differences: y is linear in x, so <dy, y(x + d) - y(x)> = <dx, d>, to the last bit here."""
+    ids = routing(T, E, kind, T + 3)
+    x, w, _, dy = data(T, E, K, N, T + 4, whole=True)
+    d = data(T, E, K, N, T + 5, whole=True)[0]
+    x = torch.where(d == 1, x.clamp(max=0), torch.where(d == -1, x.clamp(min=0), x))     # x + d stays in -1, 0, 1
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    (y, dx, dw, db), _ = oracle(x, w, None, dy, ids)
+    xd, wd, dyd = x.cuda(), w.cuda(), dy.cuda()
+    got = experts.grouped_linear(xd, wd, None, offsets, rows)
+    gx = experts.grouped_linear_dgrad(dyd, wd, offsets, rows)
+    gw, gb = experts.grouped_linear_wgrad(dyd, xd, offsets, rows)
+    assert torch.equal(got.cpu().double(), y) and torch.equal(gx.cpu().double(), dx)
+    assert torch.equal(gw.cpu().double(), dw) and torch.equal(gb.cpu().double(), db)
+    moved = experts.grouped_linear((x + d).cuda(), wd, None, offsets, rows)
+    assert ((moved.double() - got.double()) * dyd.double()).sum() == (gx.double() * d.cuda().double()).sum()
+
+
+def test_what_lies_beside_the_operands_does_not_enter():
+    """Padding behind a row, rows without an expert and experts without a row hold NaN; given results keep the rows that
+    nobody computes."""
+    T, E, K, N = 203, 5, 72, 40
+    ids = routing(T, E, 'gaps', 1)
+    x, w, b, dy = data(T, E, K, N, 2)
+    (y, dx, dw, db), (ya, dxa, dwa, dba) = oracle(x, w, b, dy, ids)
+    nan = float('nan')
+
+    def wide(t, pad):
+        buf = torch.full((*t.shape[:-1], t.shape[-1] + pad), nan, dtype=t.dtype, device='cuda')
+        buf[..., :t.shape[-1]] = t.cuda()
+        return buf[..., :t.shape[-1]]
+    gone = (ids < 0) | (ids >= E)
+    x[gone], dy[gone] = nan, nan
+    for e in range(E):
+        if not (ids == e).any():
+            w[e], b[e] = nan, nan
+    xd, wd, bd, dyd = wide(x, 8), wide(w, 24), wide(b, 4), wide(dy, 16)
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    close(experts.grouped_linear(xd, wd, bd, offsets, rows), y, ya, K + 1, 'y')
+    close(experts.grouped_linear_dgrad(dyd, wd, offsets, rows), dx, dxa, N, 'dx')
+    gw, gb = experts.grouped_linear_wgrad(dyd, xd, offsets, rows)
+    close(gw, dw, dwa, T, 'dw')
+    close(gb, db, dba, T, 'db')
+    assert experts.grouped_linear_wgrad(dyd, xd, offsets, rows, want_bias=False)[1] is None
+    for call, src, want, cols in ((experts.grouped_linear, xd, y, N), (experts.grouped_linear_dgrad, dyd, dx, K)):
+        buf = torch.full((T, cols + 8), 7.0, dtype=torch.bfloat16, device='cuda')
+        args = (src, wd, bd, offsets, rows) if call is experts.grouped_linear else (src, wd, offsets, rows)
+        assert call(*args, out=buf[:, :cols]).data_ptr() == buf.data_ptr()
+        kept = buf.cpu()
+        assert (kept[:, cols:] == 7).all() and (kept[gone] == 7).all()
+        assert not (kept[~gone][:, :cols] == 7).all()
+
+
+def test_lists_and_offsets_that_leave_the_arrays_are_cut():
+    T, E, K, N = 100, 3, 64, 16
+    x, w, b, dy = data(T, E, K, N, 3, whole=True)
+    xd, wd, dyd = x.cuda(), w.cuda(), dy.cuda()
+    rows = torch.arange(T, dtype=torch.int32)
+    rows[5], rows[70] = -4, T + 9
+    offsets = torch.tensor([-3, 40, 20, 400], dtype=torch.int32)       # expert 1 has no rows, expert 2 has 20..99
+    ids = torch.full((T,), -1)
+    ids[0:40] = 0
+    ids[20:100] = 2                                                    # rows 20..39 belong to experts 0 and 2: not compared
+    ids[5], ids[70] = -1, -1
+    clean = torch.ones(T, dtype=torch.bool)
+    clean[20:40] = False
+    (y, dx, dw, db), _ = oracle(x, w, None, dy, ids)
+    got = experts.grouped_linear(xd, wd, None, offsets.cuda(), rows.cuda(), out=torch.zeros(T, N, dtype=torch.bfloat16, device='cuda'))
+    gx = experts.grouped_linear_dgrad(dyd, wd, offsets.cuda(), rows.cuda(), out=torch.zeros(T, K, dtype=torch.bfloat16, device='cuda'))
+    gw, gb = experts.grouped_linear_wgrad(dyd, xd, offsets.cuda(), rows.cuda())
+    assert torch.equal(got.cpu().double()[clean], y[clean]) and torch.equal(gx.cpu().double()[clean], dx[clean])
+    assert torch.equal(gw[2].cpu().double(), dw[2]) and torch.equal(gb[2].cpu().double(), db[2]) and not gw[1].any()
+
+
+def test_no_rows_at_all():
+    w = torch.ones(3, 16, 24, dtype=torch.bfloat16, device='cuda')
+    offsets = torch.zeros(4, dtype=torch.int32, device='cuda')
+    x, dy = torch.empty(0, 24, dtype=torch.bfloat16, device='cuda'), torch.empty(0, 16, dtype=torch.bfloat16, device='cuda')
+    assert experts.grouped_linear(x, w, None, offsets).shape == (0, 16)
+    assert experts.grouped_linear_dgrad(dy, w, offsets).shape == (0, 24)
+    dw, db = experts.grouped_linear_wgrad(dy, x, offsets)
+    assert dw.shape == (3, 16, 24) and not dw.any() and not db.any()
+    # rows, but none with an expert
+    x = torch.full((9, 24), float('nan'), dtype=torch.bfloat16, device='cuda')
+    assert not experts.grouped_linear(x, w, None, offsets).any()
+
+
+def test_weights_inside_a_flat_buffer():
+    """Experts of one layer as ParamStore keeps them: weight and bias of an expert in turn, every tensor at a multiple of
+    64 elements."""
+    T, E, K, N = 150, 4, 72, 24
+    ids = routing(T, E, 'skewed', 5)
+    x, w, b, dy = data(T, E, K, N, 6)
+    step = (N * K + 63) // 64 * 64 + 64
+    flat = torch.full((E * step,), float('nan'), device='cuda')
+    for e in range(E):
+        flat[e * step:e * step + N * K] = w[e].float().flatten().cuda()
+        flat[e * step + step - 64:e * step + step - 64 + N] = b[e].cuda()
+    half = flat.bfloat16()
+    wv = half.as_strided((E, N, K), (step, K, 1))
+    bv = flat.as_strided((E, N), (step, 1), step - 64)
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    (y, dx, _, _), (ya, dxa, _, _) = oracle(x, w, b, dy, ids)
+    close(experts.grouped_linear(x.cuda(), wv, bv, offsets, rows), y, ya, K + 1, 'y')
+    close(experts.grouped_linear_dgrad(dy.cuda(), wv, offsets, rows), dx, dxa, N, 'dx')
+
+
+def test_another_stream_and_replayed_graphs_with_new_routing():
+    T, E, K, N = 500, 6, 128, 64
+    x, w, b, dy = [t.cuda() for t in data(T, E, K, N, 7, whole=True)]
+    ids = [routing(T, E, k, 8).cuda() for k in ('even', 'gaps', 'one')]
+    static = ids[0].clone()
+
+    def call():
+        rows, offsets = experts.expert_rows(static, E)
+        return (experts.grouped_linear(x, w, None, offsets, rows), experts.grouped_linear_dgrad(dy, w, offsets, rows),
+                *experts.grouped_linear_wgrad(dy, x, offsets, rows))
+    want = []
+    for i in ids:
+        static.copy_(i)
+        want.append([t.clone() for t in call()])
+    side = torch.cuda.Stream()
+    static.copy_(ids[1])
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = call()
+    side.synchronize()
+    assert all(torch.equal(a, c) for a, c in zip(got, want[1]))
+    graphs = []
+    for _ in range(2):                 # two graphs of the same calls: nothing of theirs is shared
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call()
+        graphs.append((graph, out))
+    for k in (2, 0, 1):
+        static.copy_(ids[k])
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        eager = call()
+        for _, out in graphs:
+            assert all(torch.equal(a, c) and torch.equal(a, d) for a, c, d in zip(out, want[k], eager))
+
+
+def test_expert_linear_and_its_gradients():
+    T, E, K, N = 257, 5, 64, 48
+    torch.manual_seed(3)
+    layer = experts.ExpertLinear(E, K, N, device='cuda')
+    ids = routing(T, E, 'gaps', 9)
+    x, _, _, dy = data(T, E, K, N, 10)
+    xd = x.cuda().requires_grad_()
+    y = layer(xd, ids.cuda())
+    y.backward(dy.cuda())
+    w, b = layer.weight.detach().bfloat16().cpu(), layer.bias.detach().cpu()
+    (ye, dx, dw, db), (ya, dxa, dwa, dba) = oracle(x, w, b, dy, ids)
+    close(y.detach(), ye, ya, K + 1, 'y')
+    close(xd.grad, dx, dxa, N, 'dx')
+    close(layer.weight.grad, dw, dwa, T, 'dw')
+    close(layer.bias.grad, db, dba, T, 'db')
+    # the gradient of a sum reaches the kernel as one expanded value; weights that changed are seen at once
+    layer.zero_grad()
+    with torch.no_grad():
+        layer.weight.mul_(2.0)
+    y2 = layer(xd, ids.cuda())
+    y2.sum().backward()
+    (ye, _, dw, _), (ya, _, dwa, _) = oracle(x, layer.weight.detach().bfloat16().cpu(), b, torch.ones(T, N), ids)
+    close(y2.detach(), ye, ya, K + 1, 'y')
+    close(layer.weight.grad, dw, dwa, T, 'dw')
+    frozen = experts.ExpertLinear(E, K, N, bias=False, device='cuda').requires_grad_(False)
+    x3 = x.cuda().requires_grad_()
+    frozen(x3, ids.cuda()).backward(dy.cuda())
+    assert x3.grad is not None and frozen.weight.grad is None
+
+
+def test_refusals():
+    T, E, K, N = 32, 3, 64, 16
+    x, w, b, dy = [t.cuda() for t in data(T, E, K, N, 11)]
+    rows, offsets = experts.expert_rows(routing(T, E, 'even', 1).cuda(), E)
+    ok = (x, w, b, offsets, rows)
+
+    def swap(i, v):
+        return tuple(v if k == i else t for k, t in enumerate(ok))
+    for bad in (swap(0, x.float()), swap(1, w.float())):
+        with pytest.raises(TypeError):
+            experts.grouped_linear(*bad)
+    for bad in (swap(0, x[:, :-8]), swap(0, x[0]), swap(0, x[:, 1:57]), swap(1, w[0]), swap(1, w[:, :12]), swap(2, b.bfloat16()),
+                swap(2, b[:2]), swap(3, offsets[:-1]), swap(3, offsets.long()), swap(4, rows[:-1]), swap(4, rows.long()),
+                swap(0, x.t().contiguous().t())):
+        with pytest.raises(ValueError):
+            experts.grouped_linear(*bad)
+    for bad in (swap(0, x.cpu()), swap(1, w.cpu())):
+        with pytest.raises(RuntimeError):
+            experts.grouped_linear(*bad)
+    with pytest.raises(ValueError):
+        experts.grouped_linear(*ok, out=torch.empty(T, N + 8, dtype=torch.bfloat16, device='cuda'))
+    with pytest.raises(ValueError):
+        experts.grouped_linear_dgrad(x, w, offsets, rows)
+    with pytest.raises(ValueError):
+        experts.grouped_linear_wgrad(dy[:-1], x, offsets, rows)
+    with pytest.raises(ValueError):
+        experts.expert_rows(rows.long(), 3)
+    for n in (0, 513):
+        with pytest.raises(ValueError):
+            experts.expert_rows(rows, n)

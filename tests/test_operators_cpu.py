@@ -46,3 +46,71 @@ def test_adamw8_needs_a_device():
 def test_noise_keys_differ_by_step_and_seed():
     keys = {optim.noise_key(s, t) for s in range(8) for t in range(1, 129)}
     assert len(keys) == 8 * 128 and all(0 <= k < 1 << 31 for k in keys)
+
+
+def grouped(entry, *more, **over):
+    from vitpose_amd._lib import GroupedArgs
+    import ctypes
+    a = dict(T=16, E=2, N=16, K=32, offsets=64, rows=64, x=64, ldx=32, w=64, ldw=32, stride_w=512, bias=64, stride_b=16, dy=64,
+             ldy=16, out=64, ldo=32, zero_rest=0)
+    a.update(over)
+    return getattr(_lib.lib(), entry)(ctypes.byref(GroupedArgs(*a.values())), *more, None)
+
+
+COMMON = [dict(T=-1), dict(E=0), dict(N=12), dict(N=0), dict(K=20), dict(offsets=None)]
+
+
+@pytest.mark.parametrize('over', COMMON + [dict(x=None), dict(x=72), dict(w=None), dict(w=66), dict(out=None), dict(out=8), dict(ldx=24),
+                                           dict(ldx=36), dict(ldw=24), dict(ldo=8), dict(ldo=20), dict(stride_w=100), dict(bias=68),
+                                           dict(stride_b=18)])
+def test_grouped_fwd_refuses_on_the_host(over):
+    assert grouped('vp_grouped_fwd', **over) == ERR_ARG
+
+
+@pytest.mark.parametrize('over', COMMON + [dict(dy=None), dict(dy=72), dict(w=None), dict(out=8), dict(ldy=8), dict(ldy=20), dict(ldo=24)])
+def test_grouped_dgrad_refuses_on_the_host(over):
+    assert grouped('vp_grouped_dgrad', **over) == ERR_ARG
+
+
+@pytest.mark.parametrize('over', COMMON + [dict(dy=None), dict(x=None), dict(x=72), dict(ldx=24), dict(ldy=12)])
+def test_grouped_wgrad_refuses_on_the_host(over):
+    assert grouped('vp_grouped_wgrad', 64, 64, None, 0, **over) == ERR_ARG
+
+
+def test_grouped_wgrad_refuses_missing_results_and_workspace():
+    assert grouped('vp_grouped_wgrad', None, 64, None, 0) == ERR_ARG
+    assert grouped('vp_grouped_wgrad', 72, 64, None, 0) == ERR_ARG
+    assert _lib.lib().vp_grouped_wgrad_slices(100000, 1, 16, 32) > 1
+    assert grouped('vp_grouped_wgrad', 64, 64, None, 0, T=100000, E=1) == ERR_ARG
+    assert grouped('vp_grouped_wgrad', 64, 64, 64, 1024, T=100000, E=1) == ERR_ARG
+
+
+def test_grouped_products_of_no_rows_touch_nothing():
+    assert grouped('vp_grouped_fwd', T=0, x=None, out=None) == 0
+    assert grouped('vp_grouped_dgrad', T=0, dy=None, out=None) == 0
+
+
+def test_expert_rows_refuses_on_the_host():
+    L = _lib.lib()
+    for a in ((64, -1, 2, 64, 64), (64, 8, 0, 64, 64), (None, 8, 2, 64, 64), (64, 8, 2, None, 64), (64, 8, 2, 64, None)):
+        assert L.vp_expert_rows(*a, None) == ERR_ARG
+    assert L.vp_expert_rows(64, 8, 513, 64, 64, None) == -2
+
+
+def test_expert_operators_need_a_device():
+    from vitpose_amd import experts
+    x, w = torch.zeros(8, 16, dtype=torch.bfloat16), torch.zeros(2, 8, 16, dtype=torch.bfloat16)
+    offsets = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        experts.expert_rows(offsets, 2)
+    with pytest.raises(RuntimeError):
+        experts.grouped_linear(x, w, None, offsets)
+    with pytest.raises(RuntimeError):
+        experts.grouped_linear_dgrad(x[:, :8], w, offsets)
+    with pytest.raises(RuntimeError):
+        experts.grouped_linear_wgrad(x, x, offsets)
+    with pytest.raises(ValueError):
+        experts.ExpertLinear(2, 12, 16)
+    with pytest.raises(ValueError):
+        experts.ExpertLinear(513, 16, 16)
+    assert set(experts.ExpertLinear(2, 16, 8).state_dict()) == {'weight', 'bias'}

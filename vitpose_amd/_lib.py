@@ -49,6 +49,13 @@ class GroupEntry(Structure):
                 ('image_mask', c_void_p), ('tiles_per_image', c_int)]
 
 
+class GroupedArgs(Structure):
+    _fields_ = [('T', c_int), ('E', c_int), ('N', c_int), ('K', c_int), ('offsets', c_void_p), ('rows', c_void_p),
+                ('x', c_void_p), ('ldx', c_long), ('w', c_void_p), ('ldw', c_long), ('stride_w', c_long),
+                ('bias', c_void_p), ('stride_b', c_long), ('dy', c_void_p), ('ldy', c_long),
+                ('out', c_void_p), ('ldo', c_long), ('zero_rest', c_int)]
+
+
 class LnPartial(Structure):
     _fields_ = [('partial', c_void_p), ('dgamma', c_void_p), ('dbeta', c_void_p), ('dcolsum', c_void_p),
                 ('blocks', c_int), ('overwrite', c_int)]
@@ -122,6 +129,11 @@ SIGNATURES = {
     'vp_pos_embed_grad': [P, P, c_int, c_int, c_int, P],
     'vp_adamw_step': [P, P, P, P, P, P, P, P, P, c_int, c_float, c_float, c_float, c_float, c_int, P,
                       c_float, c_float, P],
+    'vp_expert_rows': [P, c_int, c_int, P, P, P],
+    'vp_grouped_fwd': [POINTER(GroupedArgs), P],
+    'vp_grouped_dgrad': [POINTER(GroupedArgs), P],
+    'vp_grouped_wgrad': [POINTER(GroupedArgs), P, P, P, c_size_t, P],
+    'vp_grouped_wgrad_slices': [c_int, c_int, c_int, c_int],     # host-side helper: no stream argument
     'vp_sumsq_chunks_f64': [P, P, P, c_int, c_long, P, c_int, P],
     'vp_adamw8_step': [P] * 12 + [c_int, c_long, c_long, c_double, c_double, c_double, c_double, c_long, P, c_int,
                                   c_float, c_float, c_uint, P],
