@@ -379,6 +379,26 @@ int vp_grouped_wgrad(const vp_grouped_args* args, float* dw, float* db, void* wo
                      vp_stream_t stream);
 int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: no stream argument */
 
+/* ------------------------------------------------------- 8-bit block products ------
+ * nn.Linear (vit.py:66-74,93,96) on e4m3 (OCP, finite) operands with f32 scales, the largest magnitude of a block over 448:
+ *   quantize_rows:   x [M][ldx >= K] f32 or bf16 -> q [M][Kp], scale [Kp / 128][M]: one scale per row and 128 values of K
+ *   quantize_weight: w [N][ldw >= K] f32 or bf16 -> q [N][Kp], scale [ceil(N / 128)][Kp / 128]: one per 128 x 128 square
+ *     Kp = K rounded up to 128, the padding zeros; nearest, ties to even.  A block whose largest magnitude is under
+ *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K, ldx, ldw multiples of 8.
+ *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias), sums in f32; K = Kp,
+ *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16), bias [N] f32 or NULL, act 0: none, 1: GELU (erf).
+ * Array starts on 16 bytes. */
+typedef struct vp_fp8_args {
+    int M, N, K;
+    const void* xq; long ldx; const float* xs;
+    const void* wq; long ldw; const float* ws;
+    const float* bias; int act;
+    void* out; long ldo; int out_dtype;
+} vp_fp8_args;
+int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, int K, void* q, float* scale, vp_stream_t stream);
+int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale, vp_stream_t stream);
+int vp_gemm_fp8(const vp_fp8_args* args, vp_stream_t stream);
+
 /* --------------------------------------------------------------- Input side ------
  * vp_warp_affine_normalize: TopDownAffine's cv2.warpAffine(img, trans, image_size, INTER_LINEAR)
  *   (datasets/pipelines/top_down_transform.py:312-363) + ToTensor + NormalizeTensor (shared_transform.py:21-64)

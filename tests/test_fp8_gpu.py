@@ -1,0 +1,242 @@
+"""Block-scaled e4m3 products (vp_quantize_fp8_*, vp_gemm_fp8, vitpose_amd.fp8) against the definition in 64 bits.
+
+Tolerances (U = 2^-24, half a step of f32): a scale is one product of amax and the rounded constant 1 / 448 (2 U); the value in
+front of the rounding to e4m3 passes a reciprocal and two products (4 U), so a code is the nearest one up to that, which is half a
+spacing plus 4 U of the value; a sum over Kp products in blocks, each block's sum times the product of two scales, is off by at
+most (Kp + blocks + 4) U of the sum of the magnitudes; a bf16 result by half a step more (2^-8), the GELU's polynomial by 2.5e-5
+and its slope is at most 1.13."""
+import pytest
+import torch
+
+from vitpose_amd import fp8
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def spacing(x):
+    return torch.exp2((torch.frexp(x.abs())[1] - 1).clamp(min=-6).double() - 3)
+
+
+def padded(x):
+    return torch.nn.functional.pad(x, (0, -x.shape[1] % 128))
+
+
+def check_codes(x, q, scale):
+    """x f64 [..., 128] of one block each, q its codes' values, scale f32."""
+    amax = x.abs().amax(-1)
+    live = amax >= 2.0 ** -100
+    assert ((scale.double() - amax / 448).abs() <= 2.1 * U * amax / 448)[live].all() and not scale[~live].any() and not q[~live].any()
+    v = x[live] * 448 / amax[live][..., None]
+    assert ((q[live] - v).abs() <= spacing(v) / 2 + 6 * U * v.abs()).all()
+    # the largest magnitude is the largest code
+    assert (q[live].abs().amax(-1) == 448).all()
+
+
+SHAPES = [(1, 8), (1, 128), (3, 136), (17, 1000), (64, 384), (200, 72), (129, 1280)]
+
+
+@pytest.mark.parametrize('M,K', SHAPES + [(5000, 264)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_rows_are_rounded_block_by_block(M, K, dtype):
+    g = torch.Generator().manual_seed(M + K)
+    x = (torch.randn(M, K, generator=g) * torch.exp(4 * torch.randn(M, K, generator=g))).to(dtype)
+    x[0, :8] = 0
+    if M > 2:
+        x[1] = 0
+        x[2] *= 2.0 ** -60
+        x[2] *= 2.0 ** -60          # some blocks below 2^-100
+    q, s = fp8.quantize_rows(x.cuda())
+    kb = (K + 127) // 128
+    assert q.shape == (M, kb * 128) and s.shape == (kb, M) and q.dtype == torch.float8_e4m3fn
+    check_codes(padded(x.double()).view(M, kb, 128), q.cpu().double().view(M, kb, 128), s.cpu().t())
+    wide = torch.full((M, K + 16), float('nan'), dtype=dtype, device='cuda')
+    wide[:, :K] = x.cuda()
+    q2, s2 = fp8.quantize_rows(wide[:, :K])
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+
+
+@pytest.mark.parametrize('N,K', SHAPES + [(300, 600)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_weights_are_rounded_square_by_square(N, K, dtype):
+    g = torch.Generator().manual_seed(N + K)
+    w = (torch.randn(N, K, generator=g) * torch.exp(2 * torch.randn(N, K, generator=g))).to(dtype)
+    q, s = fp8.quantize_weight(w.cuda())
+    nb, kb = (N + 127) // 128, (K + 127) // 128
+    assert q.shape == (N, kb * 128) and s.shape == (nb, kb)
+
+    def squares(t):
+        t = torch.nn.functional.pad(t, (0, kb * 128 - t.shape[1], 0, nb * 128 - N))
+        return t.view(nb, 128, kb, 128).permute(0, 2, 1, 3).reshape(nb, kb, 128 * 128)
+    check_codes(squares(w.double()), squares(q.cpu().double()), s.cpu())
+
+
+@pytest.mark.parametrize('bad', [float('nan'), float('inf'), -float('inf')])
+def test_what_is_not_finite_marks_its_block(bad):
+    x = torch.ones(4, 384, device='cuda')
+    x[1, 200] = bad
+    q, s = fp8.quantize_rows(x)
+    assert torch.isnan(s[1, 1]) and int(torch.isnan(s).sum()) == 1
+    w = torch.ones(200, 384, device='cuda')
+    wq, ws = fp8.quantize_weight(w)
+    y = fp8.product(q, s, wq, ws)
+    assert torch.isnan(y[1]).all() and (y[[0, 2, 3]] == 384).all()
+    w[150, 300] = bad
+    wq, ws = fp8.quantize_weight(w)
+    assert torch.isnan(ws[1, 2]) and int(torch.isnan(ws).sum()) == 1
+    q, s = fp8.quantize_rows(torch.ones(4, 384, device='cuda'))
+    y = fp8.product(q, s, wq, ws)
+    assert torch.isnan(y[:, 128:]).all() and (y[:, :128] == 384).all()
+
+
+GEMMS = [(1, 1, 128), (1, 17, 256), (2, 5120, 1280), (3, 64, 136), (16, 96, 1536), (17, 130, 384), (33, 1000, 200), (64, 128, 128),
+         (65, 777, 1000), (127, 129, 640), (128, 256, 2048), (192, 1024, 1024), (257, 320, 5120), (513, 72, 264), (1001, 777, 1000),
+         (2000, 33, 8)]
+
+
+def operands(M, N, K, seed):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(M, K, generator=g) * torch.exp(torch.randn(K, generator=g))
+    w = torch.randn(N, K, generator=g) * 0.05
+    return x.bfloat16(), w, torch.randn(N, generator=g)
+
+
+def oracle(xq, xs, wq, ws, bias):
+    """(y, magnitudes) in 64 bits from the quantized operands."""
+    x = xq.cpu().double() * xs.cpu().t().double().repeat_interleave(128, 1)
+    w = wq.cpu().double() * ws.cpu().double().repeat_interleave(128, 0)[:wq.shape[0]].repeat_interleave(128, 1)
+    y, mag = x @ w.t(), x.abs() @ w.abs().t()
+    eights = [t.abs().view(t.shape[0], -1, 8).amax(2) for t in (x, w)]
+    mag += 7 * 2.0 ** -13 / ((x.shape[1] + x.shape[1] // 128 + 4) * U) * (eights[0] @ eights[1].t())     # in units of close()'s
+    return (y, mag) if bias is None else (y + bias.double(), mag + bias.double().abs())
+
+
+def close(got, want, mag, Kp, act=None):
+    tol = (Kp + Kp // 128 + 4) * U * mag
+    if act:
+        want, tol = torch.nn.functional.gelu(want), 1.13 * tol + (2.6e-5 if got.dtype == torch.bfloat16 else 4 * U * want.abs())
+    if got.dtype == torch.bfloat16:
+        tol = tol + 2.0 ** -8 * (want.abs() + tol)
+    off = (got.cpu().double() - want).abs()
+    assert torch.isfinite(got).all() and (off <= tol).all(), f'{(off / tol).max().item():.3g} of the bound'
+
+
+@pytest.mark.parametrize('M,N,K', GEMMS)
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float32])
+def test_products_match_sums_in_64_bits(M, N, K, out_dtype):
+    x, w, b = operands(M, N, K, M + N + K)
+    xq, xs = fp8.quantize_rows(x.cuda())
+    wq, ws = fp8.quantize_weight(w.cuda())
+    Kp = wq.shape[1]
+    for bias, act in ((None, None), (b, None), (b, 'gelu')):
+        want, mag = oracle(xq, xs, wq, ws, bias)
+        bd = bias.cuda() if bias is not None else None
+        got = fp8.product(xq, xs, wq, ws, bd, act=act, out_dtype=out_dtype)
+        close(got, want, mag, Kp, act)
+        # (the call that rounds x itself may add up the blocks in another order)
+        close(fp8.linear(x.cuda(), wq, ws, bd, act=act, out_dtype=out_dtype), want, mag, Kp, act)
+    x32 = x.float().cuda()
+    close(fp8.linear(x32, wq, ws, out_dtype=out_dtype), *oracle(xq, xs, wq, ws, None), Kp)
+
+
+@pytest.mark.parametrize('M,N,K', GEMMS)
+def test_whole_numbers_come_out_exactly(M, N, K):
+    """Codes of small whole numbers with scales of whole powers of two: every product and sum is exact."""
+    g = torch.Generator().manual_seed(M * N + K)
+    Kp = (K + 127) // 128 * 128
+    xq = torch.randint(-8, 9, (M, Kp), generator=g).float().to(torch.float8_e4m3fn)
+    wq = torch.randint(-8, 9, (N, Kp), generator=g).float().to(torch.float8_e4m3fn)
+    xs = torch.exp2(torch.randint(-3, 3, (Kp // 128, M), generator=g).float())
+    ws = torch.exp2(torch.randint(-3, 3, ((N + 127) // 128, Kp // 128), generator=g).float())
+    want, _ = oracle(xq, xs, wq, ws, None)
+    got = fp8.product(xq.cuda(), xs.cuda(), wq.cuda(), ws.cuda(), out_dtype=torch.float32)
+    assert torch.equal(got.cpu().double(), want)
+
+
+@pytest.mark.parametrize('M,N', [(3, 50), (40, 130), (300, 264)])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_operands_and_results_inside_larger_arrays(M, N, dtype):
+    K = 200
+    x, w, b = operands(M, N, K, 3)
+    xq, xs = fp8.quantize_rows(x.cuda())
+    wq, ws = fp8.quantize_weight(w.cuda())
+    want = fp8.product(xq, xs, wq, ws, b.cuda(), out_dtype=dtype)
+    nan = torch.full((M + N, 256 + 48), 0x7F, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn)
+    nan.view(torch.uint8)[:M, :256] = xq.view(torch.uint8)
+    nan.view(torch.uint8)[M:, :256] = wq.view(torch.uint8)
+    for pad in (8, 5):                     # rows of the result on and off 8-byte boundaries
+        out = torch.full((M, N + pad), 7.0, dtype=dtype, device='cuda')
+        got = fp8.product(nan[:M, :256], xs, nan[M:, :256], ws, b.cuda(), out=out[:, :N])
+        assert got.data_ptr() == out.data_ptr() and torch.equal(got, want) and (out[:, N:] == 7).all()
+        out.fill_(7.0)
+        lin = fp8.linear(x.cuda(), wq, ws, b.cuda(), out=out[:, :N])
+        assert (out[:, N:] == 7).all()
+        torch.testing.assert_close(lin, want, rtol=2.0 ** -7 if dtype == torch.bfloat16 else 1e-4, atol=1e-4)
+
+
+def test_no_rows():
+    wq, ws = fp8.quantize_weight(torch.ones(24, 64, device='cuda'))
+    assert fp8.linear(torch.empty(0, 64, device='cuda'), wq, ws).shape == (0, 24)
+    q, s = fp8.quantize_rows(torch.empty(0, 64, device='cuda', dtype=torch.bfloat16))
+    assert q.shape == (0, 128) and s.shape == (1, 0)
+
+
+@pytest.mark.parametrize('M', [4, 500])
+def test_another_stream_and_replayed_graphs(M):
+    x, w, b = operands(M, 200, 264, 5)
+    wq, ws = fp8.quantize_weight(w.cuda())
+    xs = [(x * k).cuda() for k in (1.0, -2.0, 0.5)]
+    bd, static = b.cuda(), xs[0].clone()
+    want = [fp8.linear(v, wq, ws, bd, act='gelu') for v in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = fp8.linear(static, wq, ws, bd, act='gelu')
+    side.synchronize()
+    assert torch.equal(got, want[0])
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fp8.linear(static, wq, ws, bd, act='gelu')
+        graphs.append((graph, out))
+    for k in (1, 2, 0, 1):
+        static.copy_(xs[k])
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[k]) for _, out in graphs)
+        assert torch.equal(fp8.linear(xs[k], wq, ws, bd, act='gelu'), want[k])
+
+
+def test_refusals():
+    x, w, b = [t.cuda() for t in operands(32, 48, 136, 6)]
+    wq, ws = fp8.quantize_weight(w)
+    xq, xs = fp8.quantize_rows(x)
+    for bad in (x.half(), x.int()):
+        with pytest.raises(TypeError):
+            fp8.quantize_rows(bad)
+    for bad in (x[0], x[:, :100], x[:, 1:129], x.t(), torch.zeros(4, 0, device='cuda')):
+        with pytest.raises(ValueError):
+            fp8.quantize_rows(bad)
+    with pytest.raises(RuntimeError):
+        fp8.quantize_rows(x.cpu())
+    with pytest.raises(ValueError):
+        fp8.quantize_weight(w[:0])
+
+    def call(**kw):
+        a = dict(xq=xq, xs=xs, wq=wq, ws=ws, bias=b)
+        a.update(kw)
+        return fp8.product(a.pop('xq'), a.pop('xs'), a.pop('wq'), a.pop('ws'), a.pop('bias'), **a)
+    for kw in (dict(xq=xq.view(torch.uint8)), dict(out_dtype=torch.float16), dict(out=torch.empty(32, 48, device='cuda').half())):
+        with pytest.raises(TypeError):
+            call(**kw)
+    for kw in (dict(xq=xq[:, :128]), dict(xq=xq[:, 16:144]), dict(xs=xs.t()), dict(xs=xs[:1]), dict(ws=ws.t()), dict(ws=ws.double()),
+               dict(bias=b[:-1]), dict(bias=b.bfloat16()), dict(act='relu'), dict(out=torch.empty(32, 49, device='cuda')),
+               dict(out=torch.empty(48, 32, device='cuda').t())):
+        with pytest.raises(ValueError):
+            call(**kw)
+    with pytest.raises(RuntimeError):
+        call(wq=wq.cpu())
+    with pytest.raises(ValueError):
+        fp8.linear(x[:, :128], wq, ws)

@@ -114,3 +114,40 @@ def test_expert_operators_need_a_device():
     with pytest.raises(ValueError):
         experts.ExpertLinear(513, 16, 16)
     assert set(experts.ExpertLinear(2, 16, 8).state_dict()) == {'weight', 'bias'}
+
+
+def fp8_gemm(**over):
+    import ctypes
+    from vitpose_amd._lib import Fp8Args
+    a = dict(M=4, N=8, K=128, xq=64, ldx=128, xs=64, wq=64, ldw=128, ws=64, bias=None, act=0, out=64, ldo=8, out_dtype=1)
+    a.update(over)
+    return _lib.lib().vp_gemm_fp8(ctypes.byref(Fp8Args(*a.values())), None)
+
+
+@pytest.mark.parametrize('over', [dict(M=-1), dict(N=0), dict(K=0), dict(K=100), dict(K=192), dict(act=2), dict(out_dtype=2), dict(xq=None),
+                                  dict(xq=68), dict(xs=None), dict(wq=None), dict(wq=65), dict(ws=None), dict(out=None), dict(out=8),
+                                  dict(ldx=112), dict(ldx=136), dict(ldw=0), dict(ldo=7)])
+def test_gemm_fp8_refuses_on_the_host(over):
+    assert fp8_gemm(**over) == ERR_ARG
+
+
+@pytest.mark.parametrize('entry', ['vp_quantize_fp8_rows', 'vp_quantize_fp8_weight'])
+def test_fp8_quantizers_refuse_on_the_host(entry):
+    f = getattr(_lib.lib(), entry)
+    ok = dict(x=64, dtype=0, ld=16, rows=2, K=16, q=64, scale=64)
+    for over in (dict(x=None), dict(x=72), dict(dtype=2), dict(ld=8), dict(ld=20), dict(rows=-1), dict(K=0), dict(K=12), dict(q=None),
+                 dict(q=72), dict(scale=None)):
+        assert f(*{**ok, **over}.values(), None) == ERR_ARG, over
+
+
+def test_fp8_of_no_rows_touches_nothing_and_needs_a_device():
+    from vitpose_amd import fp8
+    assert fp8_gemm(M=0, xq=None, out=None) == 0
+    assert _lib.lib().vp_quantize_fp8_rows(None, 0, 16, 0, 16, None, None, None) == 0
+    x = torch.zeros(4, 16)
+    with pytest.raises(RuntimeError):
+        fp8.quantize_rows(x)
+    with pytest.raises(RuntimeError):
+        fp8.quantize_weight(x)
+    with pytest.raises(RuntimeError):
+        fp8.linear(x, x, x)

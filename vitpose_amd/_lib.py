@@ -56,6 +56,12 @@ class GroupedArgs(Structure):
                 ('out', c_void_p), ('ldo', c_long), ('zero_rest', c_int)]
 
 
+class Fp8Args(Structure):
+    _fields_ = [('M', c_int), ('N', c_int), ('K', c_int), ('xq', c_void_p), ('ldx', c_long), ('xs', c_void_p),
+                ('wq', c_void_p), ('ldw', c_long), ('ws', c_void_p), ('bias', c_void_p), ('act', c_int),
+                ('out', c_void_p), ('ldo', c_long), ('out_dtype', c_int)]
+
+
 class LnPartial(Structure):
     _fields_ = [('partial', c_void_p), ('dgamma', c_void_p), ('dbeta', c_void_p), ('dcolsum', c_void_p),
                 ('blocks', c_int), ('overwrite', c_int)]
@@ -134,6 +140,9 @@ SIGNATURES = {
     'vp_grouped_dgrad': [POINTER(GroupedArgs), P],
     'vp_grouped_wgrad': [POINTER(GroupedArgs), P, P, P, c_size_t, P],
     'vp_grouped_wgrad_slices': [c_int, c_int, c_int, c_int],     # host-side helper: no stream argument
+    'vp_quantize_fp8_rows': [P, c_int, c_long, c_int, c_int, P, P, P],
+    'vp_quantize_fp8_weight': [P, c_int, c_long, c_int, c_int, P, P, P],
+    'vp_gemm_fp8': [POINTER(Fp8Args), P],
     'vp_sumsq_chunks_f64': [P, P, P, c_int, c_long, P, c_int, P],
     'vp_adamw8_step': [P] * 12 + [c_int, c_long, c_long, c_double, c_double, c_double, c_double, c_long, P, c_int,
                                   c_float, c_float, c_uint, P],
