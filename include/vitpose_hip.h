@@ -398,6 +398,11 @@ typedef struct vp_fp8_args {
 int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, int K, void* q, float* scale, vp_stream_t stream);
 int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale, vp_stream_t stream);
 int vp_gemm_fp8(const vp_fp8_args* args, vp_stream_t stream);
+/* quantize_rows and gemm in one call: x [M][ldx >= K] f32 or bf16 instead of args->xq / ldx / xs (which are not read; args->K
+ * = Kp).  One launch where few rows make one, decided by M, N, K and dtype alone (vp_linear_fp8_fused tells); otherwise xq [M][Kp] and
+ * xs [Kp / 128][M] are the caller's scratch. */
+int vp_linear_fp8(const vp_fp8_args* args, const void* x, int dtype, long ldx, int K, void* xq, float* xs, vp_stream_t stream);
+int vp_linear_fp8_fused(int M, int N, int K, int dtype);   /* host-side helper: no stream argument */
 
 /* --------------------------------------------------------------- Input side ------
  * vp_warp_affine_normalize: TopDownAffine's cv2.warpAffine(img, trans, image_size, INTER_LINEAR)

@@ -151,3 +151,31 @@ def test_fp8_of_no_rows_touches_nothing_and_needs_a_device():
         fp8.quantize_weight(x)
     with pytest.raises(RuntimeError):
         fp8.linear(x, x, x)
+
+
+def linear_fp8(**over):
+    import ctypes
+    from vitpose_amd._lib import Fp8Args
+    a = dict(M=4, N=8, K=128, xq=None, ldx=0, xs=None, wq=64, ldw=128, ws=64, bias=None, act=0, out=64, ldo=8, out_dtype=1)
+    more = dict(x=64, dtype=1, rows=16, k=16, q=64, s=64)
+    for k, v in over.items():
+        (more if k in more else a)[k] = v
+    return _lib.lib().vp_linear_fp8(ctypes.byref(Fp8Args(*a.values())), *more.values(), None)
+
+
+@pytest.mark.parametrize('over', [dict(M=-1), dict(N=0), dict(K=100), dict(wq=None), dict(wq=72), dict(ws=None), dict(out=None), dict(ldw=64),
+                                  dict(ldo=4), dict(act=5), dict(out_dtype=7), dict(x=None), dict(x=72), dict(dtype=2), dict(rows=8),
+                                  dict(rows=20), dict(k=12), dict(k=0), dict(k=136, rows=136), dict(M=100000, N=5120, q=None),
+                                  dict(M=100000, N=5120, s=None)])
+def test_linear_fp8_refuses_on_the_host(over):
+    over = dict(over)
+    if over.get('N') == 5120:
+        over['ldo'] = 5120
+    assert linear_fp8(**over) == ERR_ARG
+
+
+def test_linear_fp8_of_no_rows_touches_nothing():
+    assert linear_fp8(M=0, x=None, q=None, s=None, out=None) == 0
+    L = _lib.lib()
+    assert L.vp_linear_fp8_fused(1, 5120, 1280, 1) == 1 and L.vp_linear_fp8_fused(24576, 1280, 5120, 1) == 0
+    assert L.vp_linear_fp8_fused(0, 8, 8, 1) == 0

@@ -143,6 +143,8 @@ SIGNATURES = {
     'vp_quantize_fp8_rows': [P, c_int, c_long, c_int, c_int, P, P, P],
     'vp_quantize_fp8_weight': [P, c_int, c_long, c_int, c_int, P, P, P],
     'vp_gemm_fp8': [POINTER(Fp8Args), P],
+    'vp_linear_fp8': [POINTER(Fp8Args), P, c_int, c_long, c_int, P, P, P],
+    'vp_linear_fp8_fused': [c_int, c_int, c_int, c_int],             # host-side helper: no stream argument
     'vp_sumsq_chunks_f64': [P, P, P, c_int, c_long, P, c_int, P],
     'vp_adamw8_step': [P] * 12 + [c_int, c_long, c_long, c_double, c_double, c_double, c_double, c_long, P, c_int,
                                   c_float, c_float, c_uint, P],

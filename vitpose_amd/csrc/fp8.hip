@@ -9,13 +9,15 @@
 // the largest of the eight with 13 bits kept below its leading one (both the 16x16x32 and the 16x16x128 form; eights meet in
 // full f32).  That is 5e-5 of the result's norm on data with a wide spread, against 2e-3 for the bf16 rounding of the result
 // and 3e-2 for the rounding of the operands to e4m3.
+#include <algorithm>
+
 #include "common.h"
 #include "vitpose_hip.h"
 
 namespace {
 
 constexpr int BLK = 128;                        // values per scale = reduction steps per K tile = bytes per tile row
-constexpr int UNIT = 64 * BLK, THREADS = 256;   // a unit: 64 rows of one K tile, 8 KiB
+constexpr int UNIT = 64 * BLK;                  // 64 rows of one K tile, 8 KiB
 constexpr float kTiny = 7.888609052210118e-31f; // 2^-100: a block below it is stored as zeros (448 / amax is finite)
 
 typedef __attribute__((ext_vector_type(8))) int i32x8;
@@ -133,9 +135,9 @@ __device__ __forceinline__ void dma16(const void* src, char* lds) {
 
 // fragment: 16 rows x 128 bytes; a lane holds 32 consecutive bytes of row li (both operands use the same order of k, so
 // which k a byte of a lane stands for does not matter)
-__device__ __forceinline__ i32x8 frag(const char* tile, int f, int lane) {
-    const int g = lane >> 4, li = lane & 15, r = (f & 3) * 16 + li;
-    const char* u = tile + (f >> 2) * UNIT + r * 128;
+__device__ __forceinline__ i32x8 frag(const char* unit, int f, int lane) {
+    const int g = lane >> 4, li = lane & 15, r = f * 16 + li;
+    const char* u = unit + r * 128;
     const i32x4 lo = *reinterpret_cast<const i32x4*>(u + (((2 * g) ^ (r & 7)) << 4));
     const i32x4 hi = *reinterpret_cast<const i32x4*>(u + (((2 * g + 1) ^ (r & 7)) << 4));
     return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
@@ -183,77 +185,249 @@ __device__ __forceinline__ f32x4 load_bias(const Args& a, int j) {
     return b;
 }
 
-// 128 x 128 tile, four waves of 64 x 64, two stages of one K tile
-__global__ __launch_bounds__(THREADS, 2) void fp8_kernel(Args a, int tiles_n) {
-    __shared__ __attribute__((aligned(16))) char lds[2][4 * UNIT];
+// BM x BN tile, 2 x WN waves of BM / 2 x BN / WN.  What bounds the product is what the CUs take in together -- some 11 TB/s,
+// hits in L2 or not --, so the tile decides: a K tile of 128 x 128 brings 32 KB for 4.2 MFLOP, one of 256 x 256 64 KB for
+// 16.8.  LDS is a ring of RING units: behind the K tile being multiplied and the next one, the loads of RING - 2 U more units
+// are in flight (with none, the 256 x 256 tile waits for every burst of loads: 2 us a K tile for 0.9 of matrix instructions).
+// A lane's accumulators are in f32 units; a K tile's product starts from zero and is added with its block's scale (one FMA
+// a value: half of the matrix instructions' time, on another unit).
+template <int BM, int BN, int WN, int RING>
+__global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
+#ifdef __HIP_DEVICE_COMPILE__   // (the host pass has no buffer resources)
+    constexpr int NT = 128 * WN, UX = BM / 64, UY = BN / 64, U = UX + UY, FM = BM / 32, FN = BN / WN / 16;
+    constexpr int PER = 512 / NT;                             // sixteen-byte pieces of a unit a thread fetches
+    constexpr int XG = 4, PARTS = FM / XG;                    // fragments of x in registers at a time
+    constexpr int PITCH = FN * 32 + 16;                       // bytes of a row of a wave's result patch
+    static_assert(FM % XG == 0 && PARTS <= 2 && FN * 16 <= 64 && 64 % (FN * 16) == 0, "a wave's columns lie in one unit");
+    static_assert(RING >= 2 * U && 2 * WN * 16 * PITCH <= RING * UNIT, "two K tiles, and the patches in their place");
+    constexpr int SROWS = BM / (2 * WN), SBYTES = 2 * WN * 256;   // scales: a wave fetches SROWS rows' of a K tile
+    static_assert(SROWS <= 64, "one value a lane");
+    __shared__ __attribute__((aligned(16))) char lds[RING * UNIT + 2 * SBYTES];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave >> 1, wn = wave & 1, g = lane >> 4, li = lane & 15;
+    const int wm = wave / WN, wn = wave % WN, g = lane >> 4, li = lane & 15;
     const int work = xcd_remap(blockIdx.x, gridDim.x);
-    const int i0 = work / tiles_n * 128, j0 = work % tiles_n * 128;
+    const int i0 = work / tiles_n * BM, j0 = work % tiles_n * BN;
     const int r0 = tid >> 3, c = ((tid & 7) ^ (r0 & 7)) * 16;
-    const uint8_t* src[4][2];
+    // Buffer loads: a scalar base and K offset, one 32-bit offset a piece (rows behind the end repeat the last one: they feed
+    // what nobody stores), no 64-bit address arithmetic in the loop.
+    uint32_t off[U][PER];
 #pragma unroll
-    for (int u = 0; u < 4; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = (u & 1) * 64 + h * 32 + r0;         // rows behind the end only feed results nobody stores
-            src[u][h] = u < 2 ? a.xq + min(i0 + r, a.M - 1) * a.ldx + c : a.wq + min(j0 + r, a.N - 1) * a.ldw + c;
+        for (int h = 0; h < PER; ++h) {
+            const int r = (u < UX ? u : u - UX) * 64 + h * (NT / 8) + r0;
+            off[u][h] = u < UX ? min(r, a.M - 1 - i0) * (uint32_t)a.ldx + c : min(r, a.N - 1 - j0) * (uint32_t)a.ldw + c;
         }
-    auto stage = [&](int kb, int st) {
-        char* dst = lds[st] + wave * 1024;
+    const auto xsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xq + i0 * a.ldx), 0, -1, 0x00020000);
+    const auto wsrc = __builtin_amdgcn_make_buffer_rsrc((void*)(a.wq + j0 * a.ldw), 0, -1, 0x00020000);
+    auto load = [&](int u, int kb, int slot) {                // unit u of K tile kb (past the end: the last one again)
+        char* dst = lds + slot * UNIT + wave * 1024;
+        const int k = min(kb, a.KB - 1) * BLK;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) dma16(src[u][h] + (long)kb * BLK, dst + u * UNIT + h * 4096);
+        for (int h = 0; h < PER; ++h)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(u < UX ? xsrc : wsrc, (__attribute__((address_space(3))) void*)(dst + h * (NT * 16)),
+                                                     16, off[u][h], k, 0, 0);
     };
-    f32x4 acc[4][4];
+    f32x4 acc[FM][FN];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
-    const float* sx = a.xs;
-    const float* sw = a.ws + (long)(j0 / BLK) * a.KB;
-    int row[4];
+        for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+    // (nothing in this launch writes the scales: constant memory, so that a scalar load fetches the wave's)
+    const auto sw = (const __attribute__((address_space(4))) float*)(a.ws + (long)min((j0 + wn * FN * 16) / BLK, (a.N - 1) / BLK) * a.KB);
+    // The scales of the tile's rows go through LDS as well (two K tiles' worth): fetched into registers they would be waited for
+    // together with every load to LDS behind them.
+    const uint32_t soff = (uint32_t)min(i0 + wave * SROWS + min(lane, SROWS - 1), a.M - 1) * 4;
+    auto scales = [&](int kb) {
+        const auto src = __builtin_amdgcn_make_buffer_rsrc((void*)(a.xs + (long)min(kb, a.KB - 1) * a.M), 0, -1, 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            src, (__attribute__((address_space(3))) void*)(lds + RING * UNIT + (kb & 1) * SBYTES + wave * 256), 4, soff, 0, 0, 0);
+    };
+    scales(0);
+    float swt = sw[0];
 #pragma unroll
-    for (int m = 0; m < 4; ++m) row[m] = min(i0 + (wm * 4 + m) * 16 + li, a.M - 1);
-    stage(0, 0);
+    for (int q = 0; q < RING - U; ++q) load(q % U, q / U, q);
+    int base = 0;                                             // ring slot of the current K tile's first unit
+    auto slot = [&](int u) { const int q = base + u; return q >= RING ? q - RING : q; };
 #pragma unroll 1
     for (int t = 0; t < a.KB; ++t) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (t + 1 < a.KB) stage(t + 1, (t + 1) & 1);
-        float f[4];
-        const float swt = sw[t];
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((RING - 2 * U) * PER) : "memory");
+        __builtin_amdgcn_s_barrier();                         // K tile t has landed, K tile t - 1 has been read
+        asm volatile("" ::: "memory");
+        float f[FM];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) f[m] = sx[(long)t * a.M + row[m]] * swt;
-        const char* lx = lds[t & 1];
-        const char* ly = lds[t & 1] + 2 * UNIT;
-        i32x8 xf[4], yf[4];
+        for (int m = 0; m < FM; ++m) {
+            const int r = (wm * FM + m) * 16;
+            f[m] = *reinterpret_cast<const float*>(lds + RING * UNIT + (t & 1) * SBYTES + r / SROWS * 256 + (r % SROWS + li) * 4);
+        }
+        const char* lx0 = lds + slot(wm * (UX / 2)) * UNIT;
+        const char* lx1 = lds + slot(wm * (UX / 2) + UX / 2 - 1) * UNIT;
+        const char* ly = lds + slot(UX + wn * FN * 16 / 64) * UNIT;
+        const int yoff = wn * FN % 4;
+        i32x8 xf[XG], yf[2];
+        yf[0] = frag(ly, yoff, lane);
 #pragma unroll
-        for (int m = 0; m < 4; ++m) xf[m] = frag(lx, wm * 4 + m, lane);
+        for (int m = 0; m < XG; ++m) xf[m] = frag(lx0, m, lane);
+        scales(t + 1);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) yf[n] = frag(ly, wn * 4 + n, lane);
+        for (int q = RING - U; q < RING; ++q) load(q % U, t + q / U, slot(q));
 #pragma unroll
-        for (int m = 0; m < 4; ++m)
+        for (int m = 0; m < FM; ++m) f[m] *= swt;
+        swt = sw[min(t + 1, a.KB - 1)];
+        __builtin_amdgcn_sched_barrier(0);
+        // One matrix instruction, then the four FMAs of the one issued LAG before it: between a matrix instruction and the
+        // first use of its result there have to be eleven others, or the compiler fills up with waits.
+        constexpr int ALL = PARTS * XG * FN, LAG = 3;
+        f32x4 d[LAG + 1];
 #pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const f32x4 d = mfma_fp8(yf[n], xf[m], f32x4{0.f, 0.f, 0.f, 0.f});
+        for (int i = 0; i < ALL + LAG; ++i) {
+            const int part = i / (XG * FN), n = i / XG % FN, m = i % XG;
+            if (i < ALL) {
+                if (m == 0 && i + XG < ALL) yf[(n + 1) & 1] = frag(ly, yoff + (n + 1) % FN, lane);
+                d[i % (LAG + 1)] = mfma_fp8(yf[n & 1], xf[m], f32x4{0.f, 0.f, 0.f, 0.f});
+                if (PARTS > 1 && part == 0 && n == FN - 1) xf[m] = frag(lx1, m, lane);
+            }
+            if (i >= LAG) {
+                const int j = i - LAG, p = j / (XG * FN) * XG + j % XG, q = j / XG % FN;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[p][q][r] = fmaf(d[j % (LAG + 1)][r], f[p], acc[p][q][r]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        base = base + U >= RING ? base + U - RING : base + U;
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");          // no load may land in LDS that is used for something else
+    __syncthreads();
+    f32x4 bias[FN];
+    const int jw = j0 + wn * FN * 16, iw = i0 + wm * FM * 16;
+#pragma unroll
+    for (int n = 0; n < FN; ++n) bias[n] = load_bias(a, jw + n * 16 + g * 4);
+    if (!a.out_f32 && ((a.N | (int)a.ldo) & 7) == 0) {
+        // through a patch of LDS of the wave's own, sixteen rows at a time, so that a lane stores sixteen bytes of a row
+        constexpr int SEG = FN * 2;
+        char* patch = lds + wave * 16 * PITCH;
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+#pragma unroll
+            for (int n = 0; n < FN; ++n) {
+                const f32x4 v = finish(a, acc[m][n], bias[n]);
+                *reinterpret_cast<bf16x4*>(patch + li * PITCH + n * 32 + g * 8) = pack4(v[0], v[1], v[2], v[3]);
+            }
+#pragma unroll
+            for (int q = 0; q < SEG / 4; ++q) {
+                const int at = q * 64 + lane, r = at / SEG, i = iw + m * 16 + r, j = jw + at % SEG * 8;
+                const bf16x8 v = *reinterpret_cast<const bf16x8*>(patch + r * PITCH + at % SEG * 16);
+                if (i < a.M && j < a.N) *reinterpret_cast<bf16x8*>((bf16*)a.out + i * a.ldo + j) = v;
+            }
+        }
+        return;
+    }
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+        const int i = iw + m * 16 + li;
+        if (i >= a.M) continue;
+#pragma unroll
+        for (int n = 0; n < FN; ++n) {
+            const int j = jw + n * 16 + g * 4;
+            if (j < a.N) store4(a, i, j, finish(a, acc[m][n], bias[n]));
+        }
+    }
+#endif
+}
+
+// ---- few rows: what counts is how soon the weights have been read, by how many CUs ----
+// A workgroup computes 16 FM rows x 16 FN columns; its eight waves take every eighth block of K straight from memory into
+// matrix-instruction operands, and the eight partial tiles are added up in LDS in a fixed order.  Rows in f32 or bf16 are
+// rounded to e4m3 on the way (a block of a row lies in four lanes): the same codes and scales as the quantizer's, without
+// its launch; every workgroup of a row does it again, which few rows can afford.
+template <typename T, int FM, int FN>
+__global__ __launch_bounds__(512, 2) void fp8_narrow_kernel(Args a, const T* __restrict__ x, long ldx, int K, int tiles_n) {
+    constexpr int TM = 16 * FM, TN = 16 * FN;
+    constexpr bool CODES = sizeof(T) == 1;
+    __shared__ __attribute__((aligned(16))) float part[8][TM][TN + 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int g = lane >> 4, li = lane & 15;
+    const int work = xcd_remap(blockIdx.x, gridDim.x);
+    const int i0 = work / tiles_n * TM, j0 = work % tiles_n * TN;
+    const T* px[FM];
+    const uint8_t* pw[FN];
+    const float* ps[FM];
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+        const int row = min(i0 + m * 16 + li, a.M - 1);
+        px[m] = x + row * ldx + g * 32;
+        ps[m] = CODES ? a.xs + row : nullptr;
+    }
+#pragma unroll
+    for (int n = 0; n < FN; ++n) pw[n] = a.wq + min(j0 + n * 16 + li, a.N - 1) * a.ldw + g * 32;
+    const float* sw = a.ws + (long)(j0 / BLK) * a.KB;
+    f32x4 acc[FM][FN];
+#pragma unroll
+    for (int m = 0; m < FM; ++m)
+#pragma unroll
+        for (int n = 0; n < FN; ++n) acc[m][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int kb = wave; kb < a.KB; kb += 8) {
+        i32x8 wf[FN], xf[FM];
+        float f[FM];
+#pragma unroll
+        for (int n = 0; n < FN; ++n) wf[n] = *reinterpret_cast<const i32x8*>(pw[n] + (long)kb * BLK);
+        const float s = sw[kb];
+        if constexpr (CODES) {
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+                xf[m] = *reinterpret_cast<const i32x8*>(px[m] + (long)kb * BLK);
+                f[m] = ps[m][(long)kb * a.M] * s;
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < FM; ++m) {
+                float v[4][8];
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int k = kb * BLK + g * 32 + q * 8;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) v[q][r] = 0.f;
+                    if (k < K) load8(px[m] + (long)kb * BLK + q * 8, v[q]);
+                }
+                uint32_t top = 0;
+#pragma unroll
+                for (int q = 0; q < 4; ++q)
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) top = max(top, abs_bits(v[q][r]));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+                top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+                float inv;
+                block_scale(top, f[m], inv);
+                f[m] *= s;
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    xf[m][2 * q] = (int)pack_e4m3(v[q][0] * inv, v[q][1] * inv, v[q][2] * inv, v[q][3] * inv);
+                    xf[m][2 * q + 1] = (int)pack_e4m3(v[q][4] * inv, v[q][5] * inv, v[q][6] * inv, v[q][7] * inv);
+                }
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < FM; ++m)
+#pragma unroll
+            for (int n = 0; n < FN; ++n) {
+                const f32x4 d = mfma_fp8(wf[n], xf[m], f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
                 for (int r = 0; r < 4; ++r) acc[m][n][r] = fmaf(d[r], f[m], acc[m][n][r]);
             }
     }
-    f32x4 bias[4];
 #pragma unroll
-    for (int n = 0; n < 4; ++n) bias[n] = load_bias(a, j0 + (wn * 4 + n) * 16 + g * 4);
+    for (int m = 0; m < FM; ++m)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-        const int i = i0 + (wm * 4 + m) * 16 + li;
-        if (i >= a.M) continue;
+        for (int n = 0; n < FN; ++n) *reinterpret_cast<f32x4*>(&part[wave][m * 16 + li][n * 16 + g * 4]) = acc[m][n];
+    __syncthreads();
+    for (int q = tid; q < TM * TN / 4; q += 512) {
+        const int r = q / (TN / 4), c = q % (TN / 4) * 4, i = i0 + r, j = j0 + c;
+        if (i >= a.M || j >= a.N) continue;
+        f32x4 v = *reinterpret_cast<const f32x4*>(&part[0][r][c]);
 #pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            const int j = j0 + (wn * 4 + n) * 16 + g * 4;
-            if (j < a.N) store4(a, i, j, finish(a, acc[m][n], bias[n]));
-        }
+        for (int w = 1; w < 8; ++w) v += *reinterpret_cast<const f32x4*>(&part[w][r][c]);
+        store4(a, i, j, finish(a, v, load_bias(a, j)));
     }
 }
 
@@ -295,17 +469,129 @@ extern "C" int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N,
     VP_LAUNCH_RET();
 }
 
-extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
+namespace {
+
+int check_fp8(const vp_fp8_args* g) {
     VP_CHECK_ARG(g && g->M >= 0 && g->N >= 1 && g->K >= BLK && g->K % BLK == 0 && (g->act == 0 || g->act == 1));
     VP_CHECK_ARG(g->out_dtype == VP_F32 || g->out_dtype == VP_BF16);
     if (g->M == 0) return VP_OK;
-    VP_CHECK_ARG(g->xq && g->xs && g->wq && g->ws && g->out && aligned16(g->xq) && aligned16(g->wq) && aligned16(g->out));
-    VP_CHECK_ARG(g->ldx >= g->K && g->ldw >= g->K && g->ldo >= g->N && g->ldx % 16 == 0 && g->ldw % 16 == 0);
-    Args a{g->M, g->N, g->K / BLK, (const uint8_t*)g->xq, g->ldx, g->xs, (const uint8_t*)g->wq, g->ldw, g->ws, g->bias,
-           g->act, g->out_dtype == VP_F32, g->out, g->ldo};
-    const int tn = cdiv(g->N, 128);
-    const long grid = (long)cdiv(g->M, 128) * tn;
+    VP_CHECK_ARG(g->wq && g->ws && g->out && aligned16(g->wq) && aligned16(g->out));
+    VP_CHECK_ARG(g->ldw >= g->K && g->ldo >= g->N && g->ldw % 16 == 0);
+    return VP_OK;
+}
+
+Args make_args(const vp_fp8_args* g) {
+    return Args{g->M, g->N, g->K / BLK, (const uint8_t*)g->xq, g->ldx, g->xs, (const uint8_t*)g->wq, g->ldw, g->ws, g->bias,
+                g->act, g->out_dtype == VP_F32, g->out, g->ldo};
+}
+
+template <typename T, int FM, int FN>
+int launch_narrow(const vp_fp8_args* g, const T* x, long ldx, int K, hipStream_t stream) {
+    const int tn = cdiv(g->N, 16 * FN);
+    const long grid = (long)cdiv(g->M, 16 * FM) * tn;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
-    hipLaunchKernelGGL(fp8_kernel, dim3((unsigned)grid), dim3(THREADS), 0, stream, a, tn);
+    hipLaunchKernelGGL((fp8_narrow_kernel<T, FM, FN>), dim3((unsigned)grid), dim3(512), 0, stream, make_args(g), x, ldx, K, tn);
     VP_LAUNCH_RET();
+}
+
+template <typename T>
+int launch_narrow(int shape, const vp_fp8_args* g, const T* x, long ldx, int K, hipStream_t stream) {
+    if (shape == 0) return launch_narrow<T, 1, 1>(g, x, ldx, K, stream);
+    if (shape == 1) return launch_narrow<T, 1, 2>(g, x, ldx, K, stream);
+    if (shape == 2) return launch_narrow<T, 2, 2>(g, x, ldx, K, stream);
+    return launch_narrow<T, 2, 4>(g, x, ldx, K, stream);
+}
+
+// Which kernel: the few-rows kernels by how many operand bytes a K step costs a CU (tile rows + columns; rows that have to be
+// rounded on the way count 2.7 times, in f32 four times), a round of 256 workgroups at a time, the 128 x 128 tile the same
+// way at 0.8 of that.  Where the chip is full of them the tiles' own ratio counts: a round of 256 x 256 tiles takes 2.75 times one
+// of 128 x 128 and does four times the work (24576 x 1280 x 5120: 160 us against 201; 12288 x 4096 x 1024: 61 / 79; at 3000 x
+// 2000 x 3000, a third of a round: 32 / 34).  Measured, us at 16 / 192 / 768 / 1536 rows of K 5120, N 1280, rows given as codes:
+// 16 x 16 6.6 / 20 / 69 / 136, 16 x 32 8.9 / 16 / 55 / 102, 32 x 32 9.8 / 12 / 38 / 73, 32 x 64 15 / 17 / 30 / 57, 128 x 128 29 /
+// 32 / 33 / 34, 256 x 256 59 / 61 / 63 / 63; K 1000, N 777: 3.3 / 5.2 / 12 / 20, 3.8 / 5.2 / 9.4 / 16, 4.0 / 4.5 / 8.4 / 14, 5.1 / 5.7 /
+// 8.6 / 12, 7.9 / 12 / 12 / 13.
+enum { TILE_128 = 4, TILE_256 = 5 };
+constexpr int kRows[4] = {16, 16, 32, 32}, kCols[4] = {16, 32, 32, 64};
+
+double narrow_cost(int shape, int M, int N, double row_weight) {
+    const long wgs = (long)cdiv(M, kRows[shape]) * cdiv(N, kCols[shape]);
+    return (double)((wgs + 255) / 256) * (kRows[shape] * row_weight + kCols[shape]);
+}
+
+int best_narrow(int M, int N, double row_weight, double& cost) {
+    int best = 0;
+    cost = narrow_cost(0, M, N, row_weight);
+    for (int s = 1; s < 4; ++s) {
+        const double c = narrow_cost(s, M, N, row_weight);
+        if (c < cost) { cost = c; best = s; }
+    }
+    return best;
+}
+
+int product_kernel(int M, int N, double& cost) {
+    const int s = best_narrow(M, N, 1.0, cost);
+    const double w128 = std::max(1.0, (double)cdiv(M, 128) * cdiv(N, 128) / 256);
+    const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
+    const double tile = 205 * std::min(w128, 2.75 * w256);
+    if (cost <= tile) return s;
+    cost = tile;
+    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
+}
+
+// The few-rows kernel that rounds its rows itself, or -1: a launch of the quantizer costs about 4 us more, a unit of the costs above
+// 31 ns per 1000 of K.
+int fused_kernel(int M, int N, int K, int dtype) {
+    double fused, split;
+    const int s = best_narrow(M, N, dtype == VP_F32 ? 4.0 : 2.7, fused);
+    product_kernel(M, N, split);
+    return fused * K <= split * K + 4.0 / 31e-6 ? s : -1;
+}
+
+template <int BM, int BN, int WN, int RING>
+int launch_tile(const vp_fp8_args* g, hipStream_t stream) {
+    const int tn = cdiv(g->N, BN);
+    const long grid = (long)cdiv(g->M, BM) * tn;
+    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    hipLaunchKernelGGL((fp8_kernel<BM, BN, WN, RING>), dim3((unsigned)grid), dim3(128 * WN), 0, stream, make_args(g), tn);
+    VP_LAUNCH_RET();
+}
+
+}  // namespace
+
+extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
+    if (int rc = check_fp8(g)) return rc;
+    if (g->M == 0) return VP_OK;
+    VP_CHECK_ARG(g->xq && g->xs && aligned16(g->xq) && g->ldx >= g->K && g->ldx % 16 == 0);
+    VP_CHECK_ARG(g->ldx <= 1 << 22 && g->ldw <= 1 << 22);       // a tile's rows within 32-bit offsets
+    double cost;
+    const int which = product_kernel(g->M, g->N, cost);
+    if (which < TILE_128) return launch_narrow<uint8_t>(which, g, (const uint8_t*)g->xq, g->ldx, g->K, stream);
+    if (which == TILE_256) return launch_tile<256, 256, 4, 18>(g, stream);
+    // one workgroup a CU: eight waves; two: four waves each (3000 x 2000 x 3000: 31 us against 34; 192 x 4096 x 1024: 8.5 / 8.1)
+    if ((long)cdiv(g->M, 128) * cdiv(g->N, 128) > 256) return launch_tile<128, 128, 2, 9>(g, stream);
+    return launch_tile<128, 128, 4, 9>(g, stream);
+}
+
+extern "C" int vp_linear_fp8_fused(int M, int N, int K, int dtype) {
+    return M >= 1 && N >= 1 && K >= 1 && fused_kernel(M, N, K, dtype) >= 0;
+}
+
+extern "C" int vp_linear_fp8(const vp_fp8_args* g, const void* x, int dtype, long ldx, int K, void* xq, float* xs,
+                             hipStream_t stream) {
+    if (int rc = check_fp8(g)) return rc;
+    VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && K >= 8 && K % 8 == 0 && cdiv(K, BLK) * BLK == g->K);
+    VP_CHECK_ARG(ldx >= K && ldx % 8 == 0);
+    if (g->M == 0) return VP_OK;
+    VP_CHECK_ARG(x && aligned16(x));
+    const int shape = fused_kernel(g->M, g->N, K, dtype);
+    if (shape >= 0)
+        return dtype == VP_F32 ? launch_narrow<float>(shape, g, (const float*)x, ldx, K, stream)
+                               : launch_narrow<bf16>(shape, g, (const bf16*)x, ldx, K, stream);
+    VP_CHECK_ARG(xq && xs);
+    if (int rc = vp_quantize_fp8_rows(x, dtype, ldx, g->M, K, xq, xs, stream)) return rc;
+    vp_fp8_args p = *g;
+    p.xq = xq;
+    p.ldx = g->K;
+    p.xs = xs;
+    return vp_gemm_fp8(&p, stream);
 }

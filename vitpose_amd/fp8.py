@@ -137,9 +137,22 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
 
 
 def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
-    """act(x w^T + bias) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call."""
-    _real_matrix(x, 'x')
-    if (x.shape[1] + BLOCK - 1) // BLOCK * BLOCK != wq.shape[-1]:
+    """act(x w^T + bias) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call (one launch where the
+    rows are few; the blocks of K may then be added up in another order)."""
+    tag, ldx = _real_matrix(x, 'x')
+    dev, (M, K) = x.device, x.shape
+    ldw, N, Kp = _operand_checks(wq, ws, bias, act, dev)
+    if (K + BLOCK - 1) // BLOCK * BLOCK != Kp:
         raise ValueError(f'x {tuple(x.shape)} against wq {tuple(wq.shape)}')
-    xq, xs = quantize_rows(x)
-    return product(xq, xs, wq, ws, bias, act, out_dtype, out)
+    out, ldo = _result(M, N, out, out_dtype, dev)
+    if M and N:
+        L = _lib.lib()
+        q = s = None
+        if not L.vp_linear_fp8_fused(M, N, K, tag):
+            q = torch.empty(M * Kp, dtype=torch.uint8, device=dev)
+            s = torch.empty(Kp // BLOCK * M, dtype=torch.float32, device=dev)
+        args = Fp8Args(M, N, Kp, None, 0, None, wq.data_ptr(), ldw, ws.data_ptr(), bias.data_ptr() if bias is not None else None,
+                       _ACTS[act], out.data_ptr(), ldo, VP_F32 if out.dtype == torch.float32 else VP_BF16)
+        _lib.launch(dev, 'vp_linear_fp8', ctypes.byref(args), x.data_ptr(), tag, ldx, K, q.data_ptr() if q is not None else None,
+                    s.data_ptr() if s is not None else None)
+    return out
