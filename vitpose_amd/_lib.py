@@ -151,6 +151,8 @@ SIGNATURES = {
 }
 
 _lib = None
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch.cuda.current_device if not hasattr(torch._C, '_cuda_getDevice') else torch._C._cuda_getDevice
 
 
 def lib():
@@ -175,18 +177,18 @@ def lib():
     return L
 
 
-def launch(device, name, *args):
-    """Call one entry point on `device` (made current for the call if it is not) and on its current stream; pointers
-    are plain integers.  A non-zero status raises."""
-    fn = getattr(lib(), name)
-    index = device.index
-    if index is None or index == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index))
+def launch(index, entry, *args):
+    """Call one entry point (a name, or `lib()`'s function) on device number `index` (made current for the call if it is not)
+    and on its current stream; pointers are plain integers.  A non-zero status raises."""
+    if entry.__class__ is str:
+        entry = getattr(lib(), entry)
+    if index == _current_device():
+        rc = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+            rc = entry(*args, _raw_stream(index))
     if rc:
-        raise RuntimeError(f'{name} failed: {rc}')
+        raise RuntimeError(f'{entry.__name__} failed: {rc}')
 
 
 def exported_symbols():

@@ -19,6 +19,8 @@ from . import _lib
 from ._lib import GroupedArgs
 
 MAX_EXPERTS = 512
+_BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_NOT_PLAIN = (AttributeError, TypeError, ValueError, RuntimeError)
 
 
 def _on_device(t, what):
@@ -74,44 +76,65 @@ def expert_rows(expert, num_expert):
     experts, rows of one expert ascending, then the rows whose entry is not in [0, num_expert); rows offsets[e] up to
     offsets[e + 1] of the list are expert e's."""
     _on_device(expert, 'expert')
-    if expert.dtype != torch.int32 or expert.dim() != 1 or not expert.is_contiguous():
+    if expert.dtype is not _I32 or expert.dim() != 1 or not expert.is_contiguous():
         raise ValueError(f'expert: expected a contiguous one-dimensional int32 tensor, got {expert.dtype} {tuple(expert.shape)}')
     if not 1 <= num_expert <= MAX_EXPERTS:
         raise ValueError(f'num_expert {num_expert}: 1 to {MAX_EXPERTS} are supported')
-    rows = torch.empty_like(expert)
-    offsets = torch.empty(num_expert + 1, dtype=torch.int32, device=expert.device)
-    _lib.launch(expert.device, 'vp_expert_rows', expert.data_ptr(), expert.numel(), num_expert, rows.data_ptr(),
-                offsets.data_ptr())
+    T = expert.shape[0]
+    rows, offsets = expert.new_empty(T), expert.new_empty(num_expert + 1)
+    _lib.launch(expert.get_device(), _lib.lib().vp_expert_rows, expert.data_ptr(), T, num_expert, rows.data_ptr(), offsets.data_ptr())
     return rows, offsets
 
 
-def _product(name, src, src_cols, weight, bias, offsets, rows, out, out_cols):
-    dev, T = src.device, src.shape[0]
-    se, sn = _weight(weight, dev)
-    E, N, K = weight.shape
-    if src.shape[1] != src_cols:
-        raise ValueError(f'{tuple(src.shape)} rows against a weight of {tuple(weight.shape)}')
-    _routing(offsets, rows, E, T, dev)
-    sb = 0
-    if bias is not None:
-        if bias.dtype != torch.float32 or tuple(bias.shape) != (E, N) or bias.device != dev:
-            raise ValueError(f'bias: expected float32 [{E}, {N}] on {dev}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}')
-        sb = bias.stride(0) if E > 1 else N
-        if bias.stride(1) != 1 or sb % 4 or bias.data_ptr() % 16:
-            raise ValueError('bias: contiguous rows a multiple of 4 elements apart, on 16-byte boundaries')
+def _plain_routing(offsets, rows, E, T, d):
+    """Whether offsets and rows are what the kernels take as they are (cheap: `_routing` finds the words for what is not)."""
+    return (offsets.dtype is _I32 and offsets.shape == (E + 1,) and offsets.is_contiguous() and offsets.get_device() == d and
+            (rows is None or (rows.dtype is _I32 and rows.shape == (T,) and rows.is_contiguous() and rows.get_device() == d)))
+
+
+def _product(fwd, src, what, weight, bias, offsets, rows, out):
+    try:
+        T, C = src.shape
+        E, N, K = weight.shape
+        d, p, pw = src.get_device(), src.data_ptr(), weight.data_ptr()
+        plain = (d >= 0 and src.dtype is _BF16 and weight.dtype is _BF16 and C == (K if fwd else N) and E and N and K and
+                 not ((N | K) & 7 or (p | pw) & 15) and src.is_contiguous() and weight.is_contiguous() and
+                 weight.get_device() == d and _plain_routing(offsets, rows, E, T, d) and
+                 (bias is None or (bias.dtype is _F32 and bias.shape == (E, N) and bias.is_contiguous() and
+                                   bias.get_device() == d and not bias.data_ptr() & 15)))
+    except _NOT_PLAIN:
+        plain = False
+    if plain:
+        se, sn, sb, ld = N * K, K, N, C
+    else:
+        _on_device(src, what)
+        dev = src.device
+        ld = _matrix(src, what, None, dev)
+        se, sn = _weight(weight, dev)
+        E, N, K = weight.shape
+        T, C = src.shape
+        if C != (K if fwd else N):
+            raise ValueError(f'{what} {tuple(src.shape)} against a weight of {tuple(weight.shape)}')
+        _routing(offsets, rows, E, T, dev)
+        sb = 0
+        if bias is not None:
+            if bias.dtype != _F32 or tuple(bias.shape) != (E, N) or bias.device != dev:
+                raise ValueError(f'bias: expected float32 [{E}, {N}] on {dev}, got {bias.dtype} {tuple(bias.shape)} on {bias.device}')
+            sb = bias.stride(0) if E > 1 else N
+            if bias.stride(1) != 1 or sb % 4 or bias.data_ptr() % 16:
+                raise ValueError('bias: contiguous rows a multiple of 4 elements apart, on 16-byte boundaries')
+        d, p, pw = src.get_device(), src.data_ptr(), weight.data_ptr()
+    cols = N if fwd else K
     fresh = out is None
     if fresh:
-        out = torch.empty(T, out_cols, dtype=torch.bfloat16, device=dev)
-    ldo = out_cols if fresh else _matrix(out, 'out', out_cols, dev, T)
-    if T == 0:
-        return out
-    ld = src.stride(0) if T > 1 else src_cols
-    fwd = name == 'vp_grouped_fwd'
-    p = src.data_ptr()
-    args = GroupedArgs(T, E, N, K, offsets.data_ptr(), rows.data_ptr() if rows is not None else None,
-                       p if fwd else None, ld, weight.data_ptr(), sn, se, bias.data_ptr() if bias is not None else None, sb,
-                       None if fwd else p, ld, out.data_ptr(), ldo, fresh)
-    _lib.launch(dev, name, ctypes.byref(args))
+        out = src.new_empty((T, cols))
+    ldo = cols if fresh else _matrix(out, 'out', cols, src.device, T)
+    if T:
+        args = GroupedArgs(T, E, N, K, offsets.data_ptr(), rows.data_ptr() if rows is not None else None,
+                           p if fwd else None, ld, pw, sn, se, bias.data_ptr() if bias is not None else None, sb,
+                           None if fwd else p, ld, out.data_ptr(), ldo, fresh)
+        L = _lib.lib()
+        _lib.launch(d, L.vp_grouped_fwd if fwd else L.vp_grouped_dgrad, ctypes.byref(args))
     return out
 
 
@@ -119,37 +142,47 @@ def grouped_linear(x, weight, bias, offsets, rows=None, out=None):
     """out[t] = x[t] @ weight[e].T + bias[e] for every row t of expert e.  x bf16 [T, K], weight bf16 [E, N, K], bias f32
     [E, N] or None; offsets / rows as `expert_rows` returns them (rows None: the rows lie in the order of their experts).
     A new result has zeros in the rows that no expert takes; a given `out` keeps them as they are."""
-    _on_device(x, 'x')
-    _matrix(x, 'x', None, x.device)
-    return _product('vp_grouped_fwd', x, weight.shape[-1], weight, bias, offsets, rows, out, weight.shape[1])
+    return _product(True, x, 'x', weight, bias, offsets, rows, out)
 
 
 def grouped_linear_dgrad(dy, weight, offsets, rows=None, out=None):
     """The gradient of x: out[t] = dy[t] @ weight[e] for every row t of expert e, bf16 [T, K] (other rows as above)."""
-    _on_device(dy, 'dy')
-    _matrix(dy, 'dy', None, dy.device)
-    return _product('vp_grouped_dgrad', dy, weight.shape[1], weight, None, offsets, rows, out, weight.shape[-1])
+    return _product(False, dy, 'dy', weight, None, offsets, rows, out)
 
 
 def grouped_linear_wgrad(dy, x, offsets, rows=None, want_bias=True):
     """(dweight f32 [E, N, K], dbias f32 [E, N] or None): sums of dy[t]^T x[t] and dy[t] over every expert's rows."""
-    _on_device(x, 'x')
-    dev, T = x.device, x.shape[0]
-    ldx = _matrix(x, 'x', None, dev)
-    ldy = _matrix(dy, 'dy', None, dev, T)
-    _on_device(offsets, 'offsets')
-    E, N, K = offsets.numel() - 1, dy.shape[1], x.shape[1]
-    if E < 1:
-        raise ValueError('offsets: at least two values are needed')
-    _routing(offsets, rows, E, T, dev)
-    dw = torch.empty(E, N, K, dtype=torch.float32, device=dev)
-    db = torch.empty(E, N, dtype=torch.float32, device=dev) if want_bias else None
-    slices = _lib.lib().vp_grouped_wgrad_slices(T, E, N, K)
+    try:
+        (T, K), (T2, N) = x.shape, dy.shape
+        E = offsets.shape[0] - 1
+        d, px, py = x.get_device(), x.data_ptr(), dy.data_ptr()
+        plain = (d >= 0 and T == T2 and x.dtype is _BF16 and dy.dtype is _BF16 and N and K and E >= 1 and
+                 not ((N | K) & 7 or (px | py) & 15) and x.is_contiguous() and dy.is_contiguous() and dy.get_device() == d and
+                 _plain_routing(offsets, rows, E, T, d))
+    except _NOT_PLAIN:
+        plain = False
+    if plain:
+        ldx, ldy = K, N
+    else:
+        _on_device(x, 'x')
+        dev, T = x.device, x.shape[0]
+        ldx = _matrix(x, 'x', None, dev)
+        ldy = _matrix(dy, 'dy', None, dev, T)
+        _on_device(offsets, 'offsets')
+        E, N, K = offsets.numel() - 1, dy.shape[1], x.shape[1]
+        if E < 1:
+            raise ValueError('offsets: at least two values are needed')
+        _routing(offsets, rows, E, T, dev)
+        d, px, py = x.get_device(), x.data_ptr(), dy.data_ptr()
+    dw = x.new_empty((E, N, K), dtype=_F32)
+    db = x.new_empty((E, N), dtype=_F32) if want_bias else None
+    L = _lib.lib()
+    slices = L.vp_grouped_wgrad_slices(T, E, N, K)
     need = slices * E * N * (K + (1 if want_bias else 0)) if slices > 1 else 0
-    ws = torch.empty(need, dtype=torch.float32, device=dev) if need else None
-    args = GroupedArgs(T, E, N, K, offsets.data_ptr(), rows.data_ptr() if rows is not None else None, x.data_ptr(), ldx,
-                       None, 0, 0, None, 0, dy.data_ptr(), ldy, None, 0, 0)
-    _lib.launch(dev, 'vp_grouped_wgrad', ctypes.byref(args), dw.data_ptr(), db.data_ptr() if want_bias else None,
+    ws = x.new_empty(need, dtype=_F32) if need else None
+    args = GroupedArgs(T, E, N, K, offsets.data_ptr(), rows.data_ptr() if rows is not None else None, px, ldx,
+                       None, 0, 0, None, 0, py, ldy, None, 0, 0)
+    _lib.launch(d, L.vp_grouped_wgrad, ctypes.byref(args), dw.data_ptr(), db.data_ptr() if want_bias else None,
                 ws.data_ptr() if need else None, need * 4)
     return dw, db
 

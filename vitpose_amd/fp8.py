@@ -19,7 +19,8 @@ from . import _lib
 from ._lib import VP_BF16, VP_F32, Fp8Args
 
 BLOCK = 128
-_F8 = torch.float8_e4m3fn
+_F8, _BF16, _F32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
+_NOT_PLAIN = (AttributeError, TypeError, ValueError, RuntimeError)
 _ACTS = {None: 0, 'gelu': 1}
 
 
@@ -64,15 +65,28 @@ def _vector(t, what, shape, dev):
         raise ValueError(f'{what}: expected contiguous float32 {list(shape)}, got {t.dtype} {list(t.shape)}')
 
 
+def _rows(x):
+    """(device number, pointer, dtype tag, leading dimension) of the rows that a call rounds."""
+    try:
+        d, p = x.get_device(), x.data_ptr()
+        _, K = x.shape
+        if d >= 0 and (x.dtype is _BF16 or x.dtype is _F32) and K >= 8 and not (K & 7 or p & 15) and x.is_contiguous():
+            return d, p, VP_BF16 if x.dtype is _BF16 else VP_F32, K
+    except _NOT_PLAIN:
+        pass
+    tag, ld = _real_matrix(x, 'x')
+    return x.get_device(), x.data_ptr(), tag, ld
+
+
 def quantize_rows(x):
     """x f32 or bf16 [M, K] -> (e4m3 [M, Kp], f32 scales [Kp / 128, M])."""
-    tag, ld = _real_matrix(x, 'x')
+    d, p, tag, ld = _rows(x)
     M, K = x.shape
-    kb = (K + BLOCK - 1) // BLOCK
-    q = torch.empty(M, kb * BLOCK, dtype=_F8, device=x.device)
-    scale = torch.empty(kb, M, dtype=torch.float32, device=x.device)
+    kb = (K + 127) // BLOCK
+    q = x.new_empty((M, kb * BLOCK), dtype=_F8)
+    scale = x.new_empty((kb, M), dtype=_F32)
     if M:
-        _lib.launch(x.device, 'vp_quantize_fp8_rows', x.data_ptr(), tag, ld, M, K, q.data_ptr(), scale.data_ptr())
+        _lib.launch(d, _lib.lib().vp_quantize_fp8_rows, p, tag, ld, M, K, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -85,74 +99,91 @@ def quantize_weight(w):
     kb = (K + BLOCK - 1) // BLOCK
     q = torch.empty(N, kb * BLOCK, dtype=_F8, device=w.device)
     scale = torch.empty((N + BLOCK - 1) // BLOCK, kb, dtype=torch.float32, device=w.device)
-    _lib.launch(w.device, 'vp_quantize_fp8_weight', w.data_ptr(), tag, ld, N, K, q.data_ptr(), scale.data_ptr())
+    _lib.launch(w.get_device(), 'vp_quantize_fp8_weight', w.data_ptr(), tag, ld, N, K, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
-def _result(M, N, out, out_dtype, dev):
+def _result(M, N, out, out_dtype, like):
+    """(result, its leading dimension, dtype tag)."""
     if out is None:
-        if out_dtype not in (torch.bfloat16, torch.float32):
+        if out_dtype is not _BF16 and out_dtype is not _F32:
             raise TypeError(f'out_dtype: bfloat16 or float32, got {out_dtype}')
-        out = torch.empty(M, N, dtype=out_dtype, device=dev)
-        return out, N
-    _on_device(out, 'out', dev)
-    if out.dtype not in (torch.bfloat16, torch.float32):
+        return like.new_empty((M, N), dtype=out_dtype), N, VP_BF16 if out_dtype is _BF16 else VP_F32
+    _on_device(out, 'out', like.device)
+    if out.dtype not in (_BF16, _F32):
         raise TypeError(f'out: expected bfloat16 or float32, got {out.dtype}')
     if tuple(out.shape) != (M, N):
         raise ValueError(f'out: shape {tuple(out.shape)}, expected ({M}, {N})')
     ldo = out.stride(0) if M > 1 else N
     if out.numel() and ((out.stride(1) != 1 and N > 1) or ldo < N or out.data_ptr() % 16):
         raise ValueError('out: rows must be contiguous and start on a 16-byte boundary')
-    return out, ldo
+    return out, ldo, VP_F32 if out.dtype is _F32 else VP_BF16
 
 
-def _operand_checks(wq, ws, bias, act, dev):
-    ldw = _codes(wq, 'wq', dev)
-    N, Kp = wq.shape
-    _vector(ws, 'ws', ((N + BLOCK - 1) // BLOCK, Kp // BLOCK), dev)
-    if bias is not None:
-        _vector(bias, 'bias', (N,), dev)
+def _weights(wq, ws, bias, act, d, dev):
+    """(leading dimension of wq, N, Kp, pointer of bias); d and dev name the rows' device."""
+    try:
+        N, Kp = wq.shape
+        plain = (wq.dtype is _F8 and Kp >= BLOCK and not (Kp & 127 or wq.data_ptr() & 15) and wq.is_contiguous() and
+                 wq.get_device() == d and ws.dtype is _F32 and ws.shape == ((N + 127) // BLOCK, Kp // BLOCK) and
+                 ws.is_contiguous() and ws.get_device() == d and
+                 (bias is None or (bias.dtype is _F32 and bias.shape == (N,) and bias.is_contiguous() and bias.get_device() == d)))
+    except _NOT_PLAIN:
+        plain = False
+    ldw = Kp if plain else _codes(wq, 'wq', dev)
+    if not plain:
+        N, Kp = wq.shape
+        _vector(ws, 'ws', ((N + BLOCK - 1) // BLOCK, Kp // BLOCK), dev)
+        if bias is not None:
+            _vector(bias, 'bias', (N,), dev)
     if act not in _ACTS:
         raise ValueError(f'act {act!r}: one of {list(_ACTS)}')
-    return ldw, N, Kp
+    return ldw, N, Kp, bias.data_ptr() if bias is not None else None
 
 
 def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
     """act(xq wq^T with the blocks' scales + bias), bf16 or f32 [M, N]; operands as the quantizers return them."""
-    _on_device(xq, 'xq')
-    dev = xq.device
-    ldx = _codes(xq, 'xq', dev)
-    ldw, N, Kp = _operand_checks(wq, ws, bias, act, dev)
-    M = xq.shape[0]
-    if xq.shape[1] != Kp:
+    try:
+        d, p = xq.get_device(), xq.data_ptr()
+        M, Kx = xq.shape
+        plain = (d >= 0 and xq.dtype is _F8 and Kx >= BLOCK and not (Kx & 127 or p & 15) and xq.is_contiguous() and
+                 xs.dtype is _F32 and xs.shape == (Kx // BLOCK, M) and xs.is_contiguous() and xs.get_device() == d)
+    except _NOT_PLAIN:
+        plain = False
+    if not plain:
+        _on_device(xq, 'xq')
+        ldx = _codes(xq, 'xq', xq.device)
+        M, Kx = xq.shape
+        _vector(xs, 'xs', (Kx // BLOCK, M), xq.device)
+        d, p = xq.get_device(), xq.data_ptr()
+    else:
+        ldx = Kx
+    ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, xq.device)
+    if Kx != Kp:
         raise ValueError(f'xq {tuple(xq.shape)} against wq {tuple(wq.shape)}: Kp differs')
-    _vector(xs, 'xs', (Kp // BLOCK, M), dev)
-    out, ldo = _result(M, N, out, out_dtype, dev)
+    out, ldo, tag = _result(M, N, out, out_dtype, xs)
     if M and N:
-        args = Fp8Args(M, N, Kp, xq.data_ptr(), ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(),
-                       bias.data_ptr() if bias is not None else None, _ACTS[act], out.data_ptr(), ldo,
-                       VP_F32 if out.dtype == torch.float32 else VP_BF16)
-        _lib.launch(dev, 'vp_gemm_fp8', ctypes.byref(args))
+        args = Fp8Args(M, N, Kp, p, ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, tag)
+        _lib.launch(d, _lib.lib().vp_gemm_fp8, ctypes.byref(args))
     return out
 
 
 def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
     """act(x w^T + bias) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call (one launch where the
     rows are few; the blocks of K may then be added up in another order)."""
-    tag, ldx = _real_matrix(x, 'x')
-    dev, (M, K) = x.device, x.shape
-    ldw, N, Kp = _operand_checks(wq, ws, bias, act, dev)
-    if (K + BLOCK - 1) // BLOCK * BLOCK != Kp:
+    d, p, tag, ldx = _rows(x)
+    M, K = x.shape
+    ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, x.device)
+    if (K + 127) // BLOCK * BLOCK != Kp:
         raise ValueError(f'x {tuple(x.shape)} against wq {tuple(wq.shape)}')
-    out, ldo = _result(M, N, out, out_dtype, dev)
+    out, ldo, otag = _result(M, N, out, out_dtype, x)
     if M and N:
         L = _lib.lib()
         q = s = None
         if not L.vp_linear_fp8_fused(M, N, K, tag):
-            q = torch.empty(M * Kp, dtype=torch.uint8, device=dev)
-            s = torch.empty(Kp // BLOCK * M, dtype=torch.float32, device=dev)
-        args = Fp8Args(M, N, Kp, None, 0, None, wq.data_ptr(), ldw, ws.data_ptr(), bias.data_ptr() if bias is not None else None,
-                       _ACTS[act], out.data_ptr(), ldo, VP_F32 if out.dtype == torch.float32 else VP_BF16)
-        _lib.launch(dev, 'vp_linear_fp8', ctypes.byref(args), x.data_ptr(), tag, ldx, K, q.data_ptr() if q is not None else None,
-                    s.data_ptr() if s is not None else None)
+            scratch = x.new_empty(M * (Kp + Kp // BLOCK * 4), dtype=torch.uint8)       # codes, then scales
+            q = scratch.data_ptr()
+            s = q + M * Kp
+        args = Fp8Args(M, N, Kp, None, 0, None, wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, otag)
+        _lib.launch(d, L.vp_linear_fp8, ctypes.byref(args), p, tag, ldx, K, q, s)
     return out

@@ -58,7 +58,7 @@ def step_lr(base_lr: float, it: int, epoch: int, steps=(170, 200), gamma=0.1, wa
 # moments in 8 bits
 # ---------------------------------------------------------------------------------------------------------------
 STATE_BLOCK = 128      # state values that share one scale
-_F8 = torch.float8_e4m3fn
+_F8, _F32, _I64 = torch.float8_e4m3fn, torch.float32, torch.int64
 
 
 def new_state8(numel: int, device):
@@ -107,6 +107,43 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
     of 128, no overlaps; an entry that leaves the buffers is skipped);  step: number of this step, from 1;  noise: key
     of this step's random numbers (`noise_key`).  max_grad_norm > 0 clips the gradients of the table's elements by their
     norm first.  Everything is updated in place on the current stream; nothing synchronises."""
+    m8, ms, r8, rs = state
+    start, length, lr_scale, decay, state_start = chunks or (None,) * 5
+    b1, b2 = betas
+    try:
+        d, n, ns, nc = param.get_device(), param.shape, m8.shape, start.shape
+        (nb,) = ns
+        plain = (d >= 0 and len(n) == 1 and len(nc) == 1 and not nb & 127 and
+                 all(t.shape == sh and t.dtype is dt and t.is_contiguous() and t.get_device() == d for t, sh, dt in (
+                     (param, n, _F32), (grad, n, _F32), (m8, ns, _F8), (r8, ns, _F8), (ms, (nb >> 7,), _F32), (rs, (nb >> 7,), _F32),
+                     (start, nc, _I64), (length, nc, torch.int32), (lr_scale, nc, _F32), (decay, nc, _F32),
+                     (state_start, nc, _I64))) and
+                 (half is None or (half.shape == n and half.dtype is torch.bfloat16 and half.is_contiguous() and half.get_device() == d)))
+    except (AttributeError, TypeError, ValueError, RuntimeError):
+        plain = False
+    if not plain:
+        _check_adamw8(param, grad, state, chunks, half)
+    if step < 1 or not (0 <= b1 < 1 and 0 <= b2 < 1) or eps < 0:
+        raise ValueError(f'step {step}, betas {betas}, eps {eps}: step >= 1, betas in [0, 1) and eps >= 0 needed')
+    if not 0 <= noise < 1 << 32:
+        raise ValueError('noise is a 32-bit key')
+    d, n, ns, nc = param.get_device(), param.numel(), m8.numel(), start.numel()
+    if nc == 0:
+        return
+    L = _lib.lib()
+    partials, npart = None, 0
+    if max_grad_norm > 0:
+        npart = min(256, (nc + 3) // 4)
+        partials = param.new_empty(npart, dtype=torch.float64)
+        _lib.launch(d, L.vp_sumsq_chunks_f64, grad.data_ptr(), start.data_ptr(), length.data_ptr(), nc, n, partials.data_ptr(), npart)
+    _lib.launch(d, L.vp_adamw8_step, param.data_ptr(), grad.data_ptr(), m8.data_ptr(), ms.data_ptr(), r8.data_ptr(),
+                rs.data_ptr(), half.data_ptr() if half is not None else None, start.data_ptr(), length.data_ptr(),
+                lr_scale.data_ptr(), decay.data_ptr(), state_start.data_ptr(), nc, n, ns, lr, b1, b2, eps, step,
+                partials.data_ptr() if npart else None, npart, max_grad_norm, grad_scale, noise)
+
+
+def _check_adamw8(param, grad, state, chunks, half):
+    """The words for what `adamw8_step` cannot take."""
     dev = param.device
     if dev.type != 'cuda':
         raise RuntimeError('adamw8_step runs on a HIP device only')
@@ -130,23 +167,6 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
     _flat_arg(lr_scale, torch.float32, 'chunk lr scale', dev, nc)
     _flat_arg(decay, torch.float32, 'chunk weight decay', dev, nc)
     _flat_arg(state_start, torch.int64, 'chunk state start', dev, nc)
-    b1, b2 = betas
-    if step < 1 or not (0 <= b1 < 1 and 0 <= b2 < 1) or eps < 0:
-        raise ValueError(f'step {step}, betas {betas}, eps {eps}: step >= 1, betas in [0, 1) and eps >= 0 needed')
-    if not 0 <= noise < 1 << 32:
-        raise ValueError('noise is a 32-bit key')
-    if nc == 0:
-        return
-    partials, npart = None, 0
-    if max_grad_norm > 0:
-        npart = min(256, (nc + 3) // 4)
-        partials = torch.empty(npart, dtype=torch.float64, device=dev)
-        _lib.launch(dev, 'vp_sumsq_chunks_f64', grad.data_ptr(), start.data_ptr(), length.data_ptr(), nc, n,
-                    partials.data_ptr(), npart)
-    _lib.launch(dev, 'vp_adamw8_step', param.data_ptr(), grad.data_ptr(), m8.data_ptr(), ms.data_ptr(), r8.data_ptr(),
-                rs.data_ptr(), half.data_ptr() if half is not None else None, start.data_ptr(), length.data_ptr(),
-                lr_scale.data_ptr(), decay.data_ptr(), state_start.data_ptr(), nc, n, ns, lr, b1, b2, eps, step,
-                partials.data_ptr() if npart else None, npart, max_grad_norm, grad_scale, noise)
 
 
 class FlatAdamW:
