@@ -386,14 +386,16 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *     Kp = K rounded up to 128, the padding zeros; nearest, ties to even.  A block whose largest magnitude is under
  *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K, ldx, ldw multiples of 8.
  *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias), sums in f32; K = Kp,
- *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16), bias [N] f32 or NULL, act 0: none, 1: GELU (erf).
- * Array starts on 16 bytes. */
+ *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16, at most 2^22), bias [N] f32 or NULL, act 0: none,
+ *     1: GELU (erf); with out f32, resid [M][ldr >= N] f32 or NULL is added behind act (resid = out with ldr = ldo: in place).
+ * M at most 2^29.  Array starts on 16 bytes (of scales and bias: on their own 4). */
 typedef struct vp_fp8_args {
     int M, N, K;
     const void* xq; long ldx; const float* xs;
     const void* wq; long ldw; const float* ws;
     const float* bias; int act;
     void* out; long ldo; int out_dtype;
+    const float* resid; long ldr;
 } vp_fp8_args;
 int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, int K, void* q, float* scale, vp_stream_t stream);
 int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale, vp_stream_t stream);

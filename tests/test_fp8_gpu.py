@@ -240,3 +240,30 @@ def test_refusals():
         call(wq=wq.cpu())
     with pytest.raises(ValueError):
         fp8.linear(x[:, :128], wq, ws)
+
+
+@pytest.mark.parametrize('M,N,K', [(1, 5, 128), (3, 136, 64), (17, 130, 384), (40, 264, 1000), (300, 1000, 264), (2100, 1280, 256), (2100, 1281, 256)])
+@pytest.mark.parametrize('act', [None, 'gelu'])
+def test_a_residual_is_added_behind_the_activation(M, N, K, act):
+    x, w, b = operands(M, N, K, M + N + K)
+    g = torch.Generator().manual_seed(9)
+    r = torch.randn(M, N, generator=g).cuda()
+    xq, xs = fp8.quantize_rows(x.cuda())
+    wq, ws = fp8.quantize_weight(w.cuda())
+    bd = b.cuda()
+    for call in (lambda **k: fp8.product(xq, xs, wq, ws, bd, act=act, **k), lambda **k: fp8.linear(x.cuda(), wq, ws, bd, act=act, **k)):
+        plain = call(out_dtype=torch.float32)
+        want = plain + r                                      # one f32 sum of the same two numbers
+        assert torch.equal(call(out_dtype=torch.float32, resid=r), want)
+        wide = torch.full((M, N + 7), float('nan'), device='cuda')
+        wide[:, :N] = r
+        assert torch.equal(call(out_dtype=torch.float32, resid=wide[:, :N]), want)
+        got = call(out=wide[:, :N], resid=wide[:, :N])        # in place
+        assert torch.equal(got, want) and torch.isnan(wide[:, N:]).all()
+        with pytest.raises(TypeError):
+            call(resid=r)
+        for bad in (r.double(), r[:, :N - 1], r.t() if M != N else r[:1]):
+            with pytest.raises(ValueError):
+                call(out_dtype=torch.float32, resid=bad)
+        with pytest.raises(RuntimeError):
+            call(out_dtype=torch.float32, resid=r.cpu())

@@ -179,3 +179,8 @@ def test_linear_fp8_of_no_rows_touches_nothing():
     L = _lib.lib()
     assert L.vp_linear_fp8_fused(1, 5120, 1280, 1) == 1 and L.vp_linear_fp8_fused(24576, 1280, 5120, 1) == 0
     assert L.vp_linear_fp8_fused(0, 8, 8, 1) == 0
+
+
+@pytest.mark.parametrize('over', [dict(resid=64, ldr=8), dict(resid=64, ldr=7, out_dtype=0), dict(resid=68, ldr=8, out_dtype=0), dict(M=(1 << 29) + 1)])
+def test_fp8_residuals_and_row_counts_refused_on_the_host(over):
+    assert fp8_gemm(**over) == ERR_ARG and (over.get('M') or linear_fp8(**over) == ERR_ARG)

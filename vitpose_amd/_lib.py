@@ -59,7 +59,7 @@ class GroupedArgs(Structure):
 class Fp8Args(Structure):
     _fields_ = [('M', c_int), ('N', c_int), ('K', c_int), ('xq', c_void_p), ('ldx', c_long), ('xs', c_void_p),
                 ('wq', c_void_p), ('ldw', c_long), ('ws', c_void_p), ('bias', c_void_p), ('act', c_int),
-                ('out', c_void_p), ('ldo', c_long), ('out_dtype', c_int)]
+                ('out', c_void_p), ('ldo', c_long), ('out_dtype', c_int), ('resid', c_void_p), ('ldr', c_long)]
 
 
 class LnPartial(Structure):

@@ -1,6 +1,6 @@
 // Products of e4m3 operands with one f32 scale per block of 128:
 //
-//   y[m][n] = sum_kb  sx[kb][m] sw[n / 128][kb]  sum_{k in block kb} qx[m][k] qw[n][k]   (+ bias, GELU)
+//   y[m][n] = sum_kb  sx[kb][m] sw[n / 128][kb]  sum_{k in block kb} qx[m][k] qw[n][k]   (+ bias, GELU, + residual)
 //
 // x is cut along K (a scale per row and 128 values), w into 128 x 128 squares; scale = (largest magnitude) / 448, so the
 // largest value of a block becomes the largest e4m3 number.  K is padded to a multiple of 128 with zeros.
@@ -126,6 +126,7 @@ struct Args {
     const float* bias;
     int act, out_f32;
     void* out; long ldo;
+    const float* resid; long ldr;
 };
 
 __device__ __forceinline__ void dma16(const void* src, char* lds) {
@@ -155,9 +156,16 @@ __device__ __forceinline__ f32x4 gelu_f32(f32x4 v) {
 
 // one row's four columns j .. j + 3 (only those below N)
 __device__ __forceinline__ void store4(const Args& a, long row, int j, f32x4 v) {
-    const bool whole = j + 3 < a.N && (a.ldo & 3) == 0;
+    const bool whole = j + 3 < a.N && ((a.ldo | a.ldr) & 3) == 0;
     if (a.out_f32) {
         float* o = (float*)a.out + row * a.ldo + j;
+        if (a.resid) {                                        // (read before its place in `out`, which may be the same, is written)
+            const float* p = a.resid + row * a.ldr + j;
+            if (whole) v += *reinterpret_cast<const f32x4*>(p);
+            else
+                for (int r = 0; r < 4; ++r)
+                    if (j + r < a.N) v[r] += p[r];
+        }
         if (whole) *reinterpret_cast<f32x4*>(o) = v;
         else
             for (int r = 0; r < 4; ++r)
@@ -472,17 +480,18 @@ extern "C" int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N,
 namespace {
 
 int check_fp8(const vp_fp8_args* g) {
-    VP_CHECK_ARG(g && g->M >= 0 && g->N >= 1 && g->K >= BLK && g->K % BLK == 0 && (g->act == 0 || g->act == 1));
+    VP_CHECK_ARG(g && g->M >= 0 && g->M <= 1 << 29 && g->N >= 1 && g->K >= BLK && g->K % BLK == 0 && (g->act == 0 || g->act == 1));
     VP_CHECK_ARG(g->out_dtype == VP_F32 || g->out_dtype == VP_BF16);
     if (g->M == 0) return VP_OK;
     VP_CHECK_ARG(g->wq && g->ws && g->out && aligned16(g->wq) && aligned16(g->out));
     VP_CHECK_ARG(g->ldw >= g->K && g->ldo >= g->N && g->ldw % 16 == 0);
+    VP_CHECK_ARG(!g->resid || (g->out_dtype == VP_F32 && g->ldr >= g->N && aligned16(g->resid)));
     return VP_OK;
 }
 
 Args make_args(const vp_fp8_args* g) {
     return Args{g->M, g->N, g->K / BLK, (const uint8_t*)g->xq, g->ldx, g->xs, (const uint8_t*)g->wq, g->ldw, g->ws, g->bias,
-                g->act, g->out_dtype == VP_F32, g->out, g->ldo};
+                g->act, g->out_dtype == VP_F32, g->out, g->ldo, g->resid, g->resid ? g->ldr : 0};
 }
 
 template <typename T, int FM, int FN>

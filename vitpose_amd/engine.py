@@ -308,10 +308,13 @@ class VitRunner:
     # -- forward --
     def record_forward(self, plan: Plan, ws: Workspace, img: torch.Tensor, B: int, training: bool,
                        dp: Optional[torch.Tensor] = None, tokens_f32: Optional[torch.Tensor] = None,
-                       fold_ln: bool = False):
+                       fold_ln: bool = False, fp8: bool = False):
         """img [B,C,H,W] f32 -> returns the final token-major bf16 feature [B*T][E].
         fold_ln (evaluation only; the caller keeps the folded weights current with ensure_ln_fold): norm1 / norm2 of
-        every Block are folded into the Linear behind them (see record_forward_folded)."""
+        every Block are folded into the Linear behind them (see record_forward_folded).
+        fp8 (evaluation only; ensure_fp8 keeps the weights current): see record_forward_fp8."""
+        if fp8 and not training:
+            return self.record_forward_fp8(plan, ws, img, B, tokens_f32)
         if fold_ln and not training and self.ln_fold_supported():
             return self.record_forward_folded(plan, ws, img, B, tokens_f32)
         E, T, M, Hd = self.E, self.T, B * self.T, self.hidden
@@ -438,6 +441,75 @@ class VitRunner:
             slots = plan.gemm(hact, self.h(b + 'mlp.fc2.weight'), x, M, E, Hd, ldx=Hd, ldy=Hd, ldo=E, epilogue=RES,
                               bias=self.w(b + 'mlp.fc2.bias'), resid=xm, out2=None if last else xb,
                               ln_stats_out=None if last else st)
+        feat = ws.bf16('feat', M, E)
+        if self.cfg.get('last_norm', True):
+            plan.layernorm_fwd(x, self.w('last_norm.weight'), self.w('last_norm.bias'), feat, tokens_f32, None, None, M, E)
+        else:
+            plan.cast_f32_bf16(x, feat, M * E)
+            if tokens_f32 is not None:
+                plan.strided_cast(x, tokens_f32, (1, 1, 1, M * E), (0, 0, 0, 1))
+        self._x_last = x
+        return feat
+
+    # -- evaluation forward on 8-bit products --
+    def _fp8_buffers(self):
+        """e4m3 weights and scales of the Blocks' Linears {name: (wq, ws)}; one prep plan rebuilds them from the f32
+        masters.  (The routed fc2 of ViTMoE keeps its bf16 product.)"""
+        if getattr(self, '_fp8', None) is None:
+            E, Hd, dev = self.E, self.hidden, self.store.device
+            names = [('attn.qkv', 3 * E, E), ('attn.proj', E, E), ('mlp.fc1', Hd, E)] + ([] if self.part else [('mlp.fc2', E, Hd)])
+            prep, weights = Plan(), {}
+            for i in range(self.depth):
+                for name, N, K in names:
+                    kb = (K + 127) // 128
+                    wq = torch.empty(N, kb * 128, dtype=torch.float8_e4m3fn, device=dev)
+                    sc = torch.empty((N + 127) // 128, kb, dtype=torch.float32, device=dev)
+                    prep.quantize_fp8_weight(self.w(f'blocks.{i}.{name}.weight'), wq, sc, N, K)
+                    weights[f'blocks.{i}.{name}'] = (wq, sc)
+            self._fp8, self._fp8_version = (weights, prep), None
+        return self._fp8
+
+    def ensure_fp8(self, weights_version):
+        """Round the weights again when the f32 masters have changed since (4 x depth launches: once per weight version)."""
+        if getattr(self, '_fp8', None) is not None and self._fp8_version != weights_version:
+            self._fp8[1].run()
+            self._fp8_version = weights_version
+
+    def record_forward_fp8(self, plan: Plan, ws: Workspace, img: torch.Tensor, B: int,
+                           tokens_f32: Optional[torch.Tensor] = None):
+        """Evaluation forward with the Blocks' Linears (vit.py:66-74,93,96) as products of e4m3 operands, one f32 scale per
+        row and 128 values of the activations and per 128 x 128 square of a weight.  The patch embedding, attention, the
+        LayerNorms and the residual stream stay what they are in record_forward."""
+        E, T, M, Hd = self.E, self.T, B * self.T, self.hidden
+        H, W = self.img_hw
+        weights = self._fp8_buffers()[0]
+        kmax = (max(E, Hd) + 127) // 128
+        xq, xs = ws.get('fp8_q', (M * kmax * 128,), torch.uint8), ws.f32('fp8_s', M * kmax)
+
+        def linear(name, x, out, N, K, **more):
+            bias = self.w(name + '.bias') if self.has(name + '.bias') else None
+            plan.linear_fp8(x, *weights[name], out, M, N, K, xq, xs, bias=bias, **more)
+
+        col = ws.bf16('pe_col', M, self.Kpe)
+        plan.patch_im2col(img, col, B, self.C, H, W, self.patch, self.stride, self.pad)
+        x, xm = ws.f32('x_a', M, E), ws.f32('x_b', M, E)
+        plan.gemm(col, self.h('patch_embed.proj.weight'), x, M, E, self.Kpe, ldx=self.Kpe, ldy=self.Kpe, ldo=E,
+                  epilogue=_lib.VP_EPI_RESID_F32, bias=self.w('patch_embed.proj.bias'), pos=self.pos_comb, pos_rows=T)
+        xn, qkv = ws.bf16('xn1', M, E), ws.bf16('qkv', M, 3 * E)
+        ao, hact = ws.bf16('ao', M, E), ws.bf16('h', M, Hd)
+        for i in range(self.depth):
+            b = f'blocks.{i}.'
+            plan.layernorm_fwd(x, self.w(b + 'norm1.weight'), self.w(b + 'norm1.bias'), xn, None, None, None, M, E)
+            linear(b + 'attn.qkv', xn, qkv, 3 * E, E)
+            plan.attention_fwd(qkv, ao, None, B, self.heads, self.d, T, self.scale)
+            linear(b + 'attn.proj', ao, xm, E, E, resid=x)
+            plan.layernorm_fwd(xm, self.w(b + 'norm2.weight'), self.w(b + 'norm2.bias'), xn, None, None, None, M, E)
+            linear(b + 'mlp.fc1', xn, hact, Hd, E, gelu=True)
+            if self.part:
+                plan.gemm(hact, self.h(b + 'mlp.fc2.weight'), x, M, E, Hd, ldx=Hd, ldy=Hd, ldo=E,
+                          epilogue=_lib.VP_EPI_RESID_F32, bias=self.w(b + 'mlp.fc2.bias'), resid=xm, route=self._route(ws, B, i))
+            else:
+                linear(b + 'mlp.fc2', hact, x, E, Hd, resid=xm)
         feat = ws.bf16('feat', M, E)
         if self.cfg.get('last_norm', True):
             plan.layernorm_fwd(x, self.w('last_norm.weight'), self.w('last_norm.bias'), feat, tokens_f32, None, None, M, E)

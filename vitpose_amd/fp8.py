@@ -141,8 +141,22 @@ def _weights(wq, ws, bias, act, d, dev):
     return ldw, N, Kp, bias.data_ptr() if bias is not None else None
 
 
-def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
-    """act(xq wq^T with the blocks' scales + bias), bf16 or f32 [M, N]; operands as the quantizers return them."""
+def _residual(resid, M, N, tag, dev):
+    """(pointer, leading dimension) of the f32 [M, N] matrix that is added to an f32 result."""
+    _on_device(resid, 'resid', dev)
+    if tag != VP_F32:
+        raise TypeError('resid: the result has to be float32 too')
+    if resid.dtype is not _F32 or tuple(resid.shape) != (M, N):
+        raise ValueError(f'resid: expected float32 {[M, N]}, got {resid.dtype} {list(resid.shape)}')
+    ldr = resid.stride(0) if M > 1 else N
+    if resid.numel() and ((resid.stride(1) != 1 and N > 1) or ldr < N or resid.data_ptr() % 16):
+        raise ValueError('resid: rows must be contiguous and start on a 16-byte boundary')
+    return resid.data_ptr(), ldr
+
+
+def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
+    """act(xq wq^T with the blocks' scales + bias) (+ resid), bf16 or f32 [M, N]; operands as the quantizers return them.
+    resid (f32 results only) may be `out` itself."""
     try:
         d, p = xq.get_device(), xq.data_ptr()
         M, Kx = xq.shape
@@ -162,14 +176,16 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
     if Kx != Kp:
         raise ValueError(f'xq {tuple(xq.shape)} against wq {tuple(wq.shape)}: Kp differs')
     out, ldo, tag = _result(M, N, out, out_dtype, xs)
+    pr, ldr = _residual(resid, M, N, tag, xq.device) if resid is not None else (None, 0)
     if M and N:
-        args = Fp8Args(M, N, Kp, p, ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, tag)
+        args = Fp8Args(M, N, Kp, p, ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, tag,
+                       pr, ldr)
         _lib.launch(d, _lib.lib().vp_gemm_fp8, ctypes.byref(args))
     return out
 
 
-def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
-    """act(x w^T + bias) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call (one launch where the
+def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
+    """act(x w^T + bias) (+ resid) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call (one launch where the
     rows are few; the blocks of K may then be added up in another order)."""
     d, p, tag, ldx = _rows(x)
     M, K = x.shape
@@ -177,6 +193,7 @@ def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
     if (K + 127) // BLOCK * BLOCK != Kp:
         raise ValueError(f'x {tuple(x.shape)} against wq {tuple(wq.shape)}')
     out, ldo, otag = _result(M, N, out, out_dtype, x)
+    pr, ldr = _residual(resid, M, N, otag, x.device) if resid is not None else (None, 0)
     if M and N:
         L = _lib.lib()
         q = s = None
@@ -184,6 +201,6 @@ def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None):
             scratch = x.new_empty(M * (Kp + Kp // BLOCK * 4), dtype=torch.uint8)       # codes, then scales
             q = scratch.data_ptr()
             s = q + M * Kp
-        args = Fp8Args(M, N, Kp, None, 0, None, wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, otag)
+        args = Fp8Args(M, N, Kp, None, 0, None, wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, otag, pr, ldr)
         _lib.launch(d, L.vp_linear_fp8, ctypes.byref(args), p, tag, ldx, K, q, s)
     return out

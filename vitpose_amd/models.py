@@ -1194,6 +1194,10 @@ class TopDown(nn.Module):
         if self._engine is not None:
             # test_cfg['fold_layernorm'] (extension, bf16 evaluation only): norm1 / norm2 folded into qkv / fc1
             self._engine.fold_layernorm = bool((self.test_cfg or {}).get('fold_layernorm', False))
+            # test_cfg['fp8'] (extension): the Blocks' Linears on 8-bit products; fp32_exact excludes it
+            self._engine.fp8 = bool((self.test_cfg or {}).get('fp8', False))
+            if self._engine.fp8 and ((self.test_cfg or {}).get('fp32_exact') or self._engine.fold_layernorm):
+                raise ValueError("test_cfg: 'fp8' excludes 'fp32_exact' and 'fold_layernorm'")
         return bool((self.test_cfg or {}).get('fp32_exact', False))
 
     def _infer_heatmap(self, img, flip_pairs=None, img_metas=None):

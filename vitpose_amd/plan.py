@@ -485,6 +485,27 @@ class Plan:
         _chk(img, torch.float32, 'img')
         self._add('vp_patch_im2col', _p(img), _p(col), B, C, H, W, patch, stride, pad, keep=(img, col))
 
+    # -- 8-bit evaluation (see vitpose_amd/fp8.py) --
+    def quantize_fp8_weight(self, w, wq, ws, N, K):
+        """wq e4m3 [N][Kp], ws f32 [ceil(N / 128)][Kp / 128] of w f32 [N][K]."""
+        _chk(w, torch.float32, 'w'), _chk(wq, torch.float8_e4m3fn, 'wq'), _chk(ws, torch.float32, 'ws')
+        kb = (K + 127) // 128
+        assert wq.numel() >= N * kb * 128 and ws.numel() >= (N + 127) // 128 * kb
+        self._add('vp_quantize_fp8_weight', _p(w), _lib.VP_F32, K, N, K, _p(wq), _p(ws), keep=(w, wq, ws))
+
+    def linear_fp8(self, x, wq, ws, out, M, N, K, xq, xs, bias=None, gelu=False, resid=None):
+        """out (bf16, or f32 with an optional f32 resid) [M][N] = x w^T + bias, x bf16 [M][K] rounded to e4m3 on the way;
+        xq (uint8, M * Kp) and xs (f32, M * Kp / 128): scratch."""
+        _chk(x, torch.bfloat16, 'x'), _chk(xq, torch.uint8, 'xq'), _chk(xs, torch.float32, 'xs')
+        kb = (K + 127) // 128
+        assert x.numel() >= M * K and out.numel() >= M * N and xq.numel() >= M * kb * 128 and xs.numel() >= M * kb
+        assert wq.dtype == torch.float8_e4m3fn and wq.numel() >= N * kb * 128 and ws.numel() >= (N + 127) // 128 * kb
+        assert resid is None or (out.dtype == resid.dtype == torch.float32 and resid.numel() >= M * N)
+        args = _lib.Fp8Args(M, N, kb * 128, None, 0, None, _p(wq), kb * 128, _p(ws), _p(bias), int(gelu), _p(out), N,
+                            _lib.VP_F32 if out.dtype == torch.float32 else _lib.VP_BF16, _p(resid), N)
+        self._add('vp_linear_fp8', ctypes.byref(args), _p(x), _lib.VP_BF16, K, K, _p(xq), _p(xs),
+                  keep=(args, x, wq, ws, out, xq, xs, bias, resid))
+
     # -- fp32-accurate path (hi / lo pair arrays; the products are gemm(..., split3=True)) --
     def split_pair(self, x, pair, n):
         _chk(x, torch.float32, 'x'), _chk(pair, torch.bfloat16, 'pair')
