@@ -145,7 +145,7 @@ int vp_splitk_reduce(const float* slab, int nsplit, long stride, size_t n, float
                      vp_stream_t stream);
 
 /* dtype tags for the layout/cast helpers */
-enum { VP_F32 = 0, VP_BF16 = 1 };
+enum { VP_F32 = 0, VP_BF16 = 1, VP_E4M3 = 2 };
 
 /* ------------------------------------------------------------- LayerNorm --------
  * nn.LayerNorm(E, eps=1e-6) over the channel axis of token-major x [M][E] f32
@@ -388,6 +388,10 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias), sums in f32; K = Kp,
  *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16, at most 2^22), bias [N] f32 or NULL, act 0: none,
  *     1: GELU (erf); with out f32, resid [M][ldr >= N] f32 or NULL is added behind act (resid = out with ldr = ldo: in place).
+ *     out_dtype VP_E4M3: out [M][ldo >= Np] becomes the codes and oscale [Np / 128][M] the scales that quantize_rows makes
+ *     of the result (Np = N rounded up to 128, ldo a multiple of 16, no resid): the next product's rows.
+ *   layernorm_fp8: q, scale as quantize_rows makes them of (x - mean) / sqrt(var + eps) gamma + beta (norm1 / norm2,
+ *     vit.py:118-140), x [M][E] f32, E a multiple of 8, at most 2048.
  * M at most 2^29.  Array starts on 16 bytes (of scales and bias: on their own 4). */
 typedef struct vp_fp8_args {
     int M, N, K;
@@ -396,11 +400,14 @@ typedef struct vp_fp8_args {
     const float* bias; int act;
     void* out; long ldo; int out_dtype;
     const float* resid; long ldr;
+    float* oscale;
 } vp_fp8_args;
 int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, int K, void* q, float* scale, vp_stream_t stream);
+int vp_layernorm_fp8(const float* x, const float* gamma, const float* beta, float eps, int M, int E, void* q, float* scale,
+                     vp_stream_t stream);
 int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale, vp_stream_t stream);
 int vp_gemm_fp8(const vp_fp8_args* args, vp_stream_t stream);
-/* quantize_rows and gemm in one call: x [M][ldx >= K] f32 or bf16 instead of args->xq / ldx / xs (which are not read; args->K
+/* quantize_rows and gemm (not to codes) in one call: x [M][ldx >= K] f32 or bf16 instead of args->xq / ldx / xs (which are not read; args->K
  * = Kp).  One launch where few rows make one, decided by M, N, K and dtype alone (vp_linear_fp8_fused tells); otherwise xq [M][Kp] and
  * xs [Kp / 128][M] are the caller's scratch. */
 int vp_linear_fp8(const vp_fp8_args* args, const void* x, int dtype, long ldx, int K, void* xq, float* xs, vp_stream_t stream);

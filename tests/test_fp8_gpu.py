@@ -267,3 +267,101 @@ def test_a_residual_is_added_behind_the_activation(M, N, K, act):
                 call(out_dtype=torch.float32, resid=bad)
         with pytest.raises(RuntimeError):
             call(out_dtype=torch.float32, resid=r.cpu())
+
+
+def check_rounded(want, mag, Kp, q, scale, act=None):
+    """Codes and scales of a product's result against the exact result: the result itself is off by close()'s bound (before its
+    rounding to 16 bits), a scale by its block's largest such error and 2 U, a code by half a spacing and that error in its units."""
+    tol = (Kp + Kp // 128 + 4) * U * mag
+    if act:
+        want, tol = torch.nn.functional.gelu(want), 1.13 * tol + 2.6e-5
+    M, N = want.shape
+    x, t = [padded(v).view(M, -1, 128) for v in (want, tol)]
+    check_codes_within(x, t, q, scale)
+    assert not q.cpu().double()[:, N:].any()
+
+
+def check_codes_within(x, t, q, scale):
+    """x f64 [M, blocks, 128], known to t."""
+    M, kb, _ = x.shape
+    assert q.shape == (M, kb * 128) and scale.shape == (kb, M) and torch.isfinite(scale).all()
+    got, s = q.cpu().double().view(M, kb, 128), scale.cpu().t().double()
+    amax, tmax = x.abs().amax(-1), t.amax(-1)
+    assert ((s - amax / 448).abs() <= (tmax + 2.1 * U * amax) / 448).all()
+    safe = s.clamp(min=1e-30)[..., None]
+    v, e = x / safe, t / safe
+    assert ((got - v).abs() <= spacing(v.abs() + e) / 2 + e + 6 * U * v.abs()).all()
+    assert (got.abs().amax(-1)[s > 0] == 448).all()
+
+
+def check_layernorm(x, gamma, beta, q, scale, eps=1e-6):
+    """x f64.  A mean of E values in f32 is off by (E + 2) U of their mean magnitude A, so a difference from it by that and U of
+    itself; the standard deviation s, from a sum of squares, by (E / 2 + 4) U of itself and the mean's error; then come four products
+    and a sum.  Together under (E + 10) U (2 A / s + |z|) |gamma| + 2 U |result| in the result."""
+    E = x.shape[1]
+    mean, var = x.mean(1, keepdim=True), x.var(1, unbiased=False, keepdim=True)
+    sd = (var + eps).sqrt()
+    z = (x - mean) / sd
+    want = z * gamma.double() + beta.double()
+    tol = (E + 10) * U * (2 * x.abs().mean(1, keepdim=True) / sd + z.abs()) * gamma.double().abs() + 2 * U * (want.abs() + beta.double().abs())
+    check_codes_within(*[padded(v).view(len(x), -1, 128) for v in (want, tol)], q, scale)
+    assert not q.cpu().double()[:, E:].any()
+
+
+@pytest.mark.parametrize('M,E', [(1, 8), (3, 64), (5, 384), (17, 520), (64, 768), (9, 1024), (130, 1280), (7, 1536), (33, 2048), (9000, 72)])
+def test_layernorm_in_front_of_the_rounding(M, E):
+    g = torch.Generator().manual_seed(M + E)
+    x = torch.randn(M, E, generator=g) * torch.exp(torch.randn(M, 1, generator=g)) + 3 * torch.randn(M, 1, generator=g)
+    gamma, beta = 1 + 0.5 * torch.randn(E, generator=g), 0.3 * torch.randn(E, generator=g)
+    if M > 2:
+        x[2] = 1.5                          # no variance: the bias is left
+    q, s = fp8.layernorm_rows(x.cuda(), gamma.cuda(), beta.cuda())
+    check_layernorm(x.double(), gamma, beta, q, s)
+    if M > 1:
+        x[1, E // 2] = float('nan')
+        q2, s2 = fp8.layernorm_rows(x.cuda(), gamma.cuda(), beta.cuda())
+        assert torch.isnan(s2[:, 1]).all() and torch.equal(s2[:, 0], s[:, 0]) and torch.equal(s2[:, 2:], s[:, 2:])
+
+
+@pytest.mark.parametrize('M,N,K', [(1, 8, 128), (17, 130, 384), (130, 128, 64), (257, 777, 264), (300, 1000, 1000), (600, 72, 256), (4100, 1281, 136)])
+@pytest.mark.parametrize('act', [None, 'gelu'])
+def test_a_result_as_codes_for_the_next_product(M, N, K, act):
+    x, w, b = operands(M, N, K, M + N + K)
+    xq, xs = fp8.quantize_rows(x.cuda())
+    wq, ws = fp8.quantize_weight(w.cuda())
+    bd = b.cuda()
+    if N > 200:
+        bd[128:256] = 0
+        wq.view(torch.uint8)[128:256] = 0   # a block of zeros
+    q, s = fp8.product(xq, xs, wq, ws, bd, act=act, out_dtype=torch.float8_e4m3fn)
+    want, mag = oracle(xq, xs, wq, ws, bd.cpu())
+    check_rounded(want, mag, wq.shape[1], q, s, act)
+    if N > 200:
+        # the GELU's polynomial may give up to 2.5e-5 at zero, so its scale up to that over 448 (and two roundings)
+        assert (s[1] <= 2.6e-5 / 448).all() if act else not s[1].any()
+    q2, s2 = fp8.linear(x.cuda(), wq, ws, bd, act=act, out_dtype=torch.float8_e4m3fn)
+    assert torch.equal(q2.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s2, s)
+    # and the next product takes it
+    w2q, w2s = fp8.quantize_weight(torch.randn(40, N + -N % 8, generator=torch.Generator().manual_seed(1)).cuda())
+    close(fp8.product(q, s, w2q, w2s), *oracle(q, s, w2q, w2s, None), w2q.shape[1])
+    xs[0, 0] = float('nan')
+    q, s = fp8.product(xq, xs, wq, ws, bd, act=act, out_dtype=torch.float8_e4m3fn)
+    assert torch.isnan(s[:, 0]).all() and torch.isfinite(s[:, 1:]).all()
+    with pytest.raises(ValueError):
+        fp8.product(xq, xs, wq, ws, out_dtype=torch.float8_e4m3fn, resid=torch.zeros(M, N, device='cuda'))
+    with pytest.raises(ValueError):
+        fp8.linear(x.cuda(), wq, ws, out_dtype=torch.float8_e4m3fn, out=torch.zeros(M, N, device='cuda'))
+
+
+def test_layernorm_refusals():
+    x, w = torch.zeros(4, 64, device='cuda'), torch.ones(64, device='cuda')
+    assert fp8.layernorm_rows(x[:0], w, w)[0].shape == (0, 128)
+    with pytest.raises(TypeError):
+        fp8.layernorm_rows(x.bfloat16(), w, w)
+    wide = torch.ones(2056, device='cuda')
+    for bad in ((x[:, :32], w[:32], w[:32]), (x, w[:32], w), (x, w, w.bfloat16()), (torch.zeros(2, 2056, device='cuda'), wide, wide),
+                (x, torch.ones(65, device='cuda')[1:], w)):
+        with pytest.raises(ValueError):
+            fp8.layernorm_rows(*bad)
+    with pytest.raises(RuntimeError):
+        fp8.layernorm_rows(x, w.cpu(), w)

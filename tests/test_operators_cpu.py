@@ -184,3 +184,50 @@ def test_linear_fp8_of_no_rows_touches_nothing():
 @pytest.mark.parametrize('over', [dict(resid=64, ldr=8), dict(resid=64, ldr=7, out_dtype=0), dict(resid=68, ldr=8, out_dtype=0), dict(M=(1 << 29) + 1)])
 def test_fp8_residuals_and_row_counts_refused_on_the_host(over):
     assert fp8_gemm(**over) == ERR_ARG and (over.get('M') or linear_fp8(**over) == ERR_ARG)
+
+
+@pytest.mark.parametrize('over', [dict(oscale=None), dict(ldo=120), dict(ldo=136), dict(N=136), dict(resid=64)])
+def test_fp8_results_as_codes_refused_on_the_host(over):
+    a = dict(out_dtype=2, ldo=128, resid=None, ldr=8, oscale=64)
+    a.update(over)
+    assert fp8_gemm(**a) == ERR_ARG
+    assert linear_fp8(**dict(a, ldo=128, N=8, resid=None, oscale=64)) == ERR_ARG
+
+
+@pytest.mark.parametrize('over', [dict(x=None), dict(x=4), dict(gamma=None), dict(gamma=8), dict(beta=None), dict(beta=4), dict(M=-1), dict(M=1 << 30), dict(E=0),
+                                  dict(E=12), dict(E=2056), dict(q=None), dict(q=8), dict(s=None)])
+def test_layernorm_fp8_refuses_on_the_host(over):
+    a = dict(x=64, gamma=64, beta=64, eps=1e-6, M=4, E=64, q=64, s=64)
+    a.update(over)
+    assert _lib.lib().vp_layernorm_fp8(*a.values(), None) == ERR_ARG
+
+
+def test_layernorm_fp8_of_no_rows_touches_nothing():
+    assert _lib.lib().vp_layernorm_fp8(None, None, None, 1e-6, 0, 64, None, None, None) == 0
+
+
+def test_every_entry_is_called_with_the_header_s_arguments():
+    """Number and kind of the arguments in the ctypes table against the prototypes: a missing one would hand the callee a truncated
+    pointer."""
+    import ctypes
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(__file__), '..', 'include', 'vitpose_hip.h')) as f:
+        text = re.sub(r'/\*.*?\*/', '', f.read(), flags=re.S)
+    kinds = {'int': ctypes.c_int, 'long': ctypes.c_long, 'size_t': ctypes.c_size_t, 'float': ctypes.c_float, 'double': ctypes.c_double}
+    checked = 0
+    for name, params in re.findall(r'\bint (vp_\w+)\(([^;{]*)\);', text):
+        types = _lib.SIGNATURES.get(name)
+        if types is None:
+            continue
+        params = [p.strip() for p in params.split(',') if p.strip() not in ('', 'void')]
+        assert len(types) == len(params), f'{name}: {len(types)} arguments, {len(params)} in the header'
+        for t, p in zip(types, params):
+            plain = '*' not in p and '[' not in p and not p.startswith('vp_stream_t')
+            words = [w for w in p.split()[:-1] if w not in ('const', 'unsigned')]
+            if plain and words and words[0] in kinds and 'unsigned' not in p:
+                assert t is kinds[words[0]], f'{name}: {p} is called with {t.__name__}'
+            elif not plain:
+                assert ctypes.sizeof(t) == ctypes.sizeof(ctypes.c_void_p), f'{name}: {p}'
+        checked += 1
+    assert checked > 40

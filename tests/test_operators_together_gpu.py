@@ -9,7 +9,7 @@ test_fp8_gpu."""
 import pytest
 import torch
 
-from test_fp8_gpu import close, oracle as fp8_oracle
+from test_fp8_gpu import check_layernorm, check_rounded, close, oracle as fp8_oracle
 from test_model_gpu import TOY, make_engine, relerr
 
 from oracle import vitpose_oracle as O
@@ -106,15 +106,15 @@ def test_an_expert_ffn_trains_a_step_and_answers_in_8_bits(T, E, K, Hd, N):
             close(got, *fp8_oracle(xq, xs, wq, ws, layers[0].bias.detach()[e].cpu()), wq.shape[1], 'gelu')
 
 
-def test_a_vit_trained_with_8_bit_moments_evaluates_on_8_bit_products():
+@pytest.mark.parametrize('B', [2, 24])
+def test_a_vit_trained_with_8_bit_moments_evaluates_on_8_bit_products(B):
     hc = O.classic_head_cfg(64)
     eng = make_engine(TOY, hc, O.synth_vit_weights(TOY, seed=1), O.synth_head_weights(hc, seed=2), 'cuda:0')
-    B = 2
     img, target, tw = O.synth_batch(B, seed=3)
     img = img.cuda()
     old = eng.infer(img, fp8=True)
     eng.setup_optimizer(lr=1e-3, state_bits=8, noise_seed=1)
-    eng.forward_backward(img, target.cuda(), tw.cuda())
+    eng.forward_backward(img[:2], target[:2].cuda(), tw[:2].cuda())
     eng.optimizer_step()
     heat = eng.infer(img, fp8=True)
     assert not torch.equal(heat, old) and eng.optimizer.step_count == 1
@@ -126,30 +126,43 @@ def test_a_vit_trained_with_8_bit_moments_evaluates_on_8_bit_products():
         q, s = fp8.quantize_weight(eng.store.view('backbone.' + name + '.weight'))
         assert torch.equal(q.view(torch.uint8), wq.view(torch.uint8)) and torch.equal(s, ws)
 
-    # call by call: what the 8-bit products got and gave
+    # call by call: what the LayerNorms and the 8-bit products got and gave
     plan, _, out = eng.plans[('infer', B, 'fp8')]
-    buf = eng.ws_infer.bufs
-    E, M = TOY['embed_dim'], B * 192
-    stages = [('attn.qkv', 'xn1', 'qkv', None), ('attn.proj', 'ao', 'x_b', 'x_a'), ('mlp.fc1', 'xn1', 'h', None), ('mlp.fc2', 'h', 'x_a', 'x_b')]
-    seen = 0
+    buf, vit = eng.ws_infer.bufs, eng.vit
+    E, M, Hd = TOY['embed_dim'], B * 192, 4 * TOY['embed_dim']
+    rows = lambda q, s, K: (buf[q][:M * -(-K // 128) * 128].view(M, -1).view(torch.float8_e4m3fn).clone(),  # noqa: E731
+                            buf[s][:M * -(-K // 128)].view(-1, M).clone())
+    few = bool(plan.L.vp_linear_fp8_fused(M, E, Hd, 1))
+    stages = [('norm1', 'x_a'), ('attn.qkv', 'qkv', None), ('attn.proj', 'x_b', 'x_a'), ('norm2', 'x_b'),
+              ('mlp.fc1', 'h' if few else None, None), ('mlp.fc2', 'x_a', 'x_b')]
+    seen, codes = 0, None
     for i, (entry, _, _) in enumerate(plan.calls):
-        if entry != 'vp_linear_fp8':
+        if not entry.endswith('_fp8'):
             plan.run(i, i + 1)
             continue
-        block, stage = divmod(seen, 4)
-        name, src, dst, res = stages[stage]
-        x, r = buf[src].clone(), buf[res].clone() if res else None
-        plan.run(i, i + 1)
-        wq, ws = weights[f'blocks.{block}.{name}']
-        xq, xs = fp8.quantize_rows(x)
-        want, mag = fp8_oracle(xq, xs, wq, ws, eng.vit.w(f'blocks.{block}.{name}.bias').cpu())
-        got = buf[dst]
-        assert x.shape[0] == M and got.dtype == (torch.float32 if res else torch.bfloat16)
-        if res:
-            want, mag = want + r.cpu().double(), mag + r.cpu().double().abs()
-        close(got, want, mag, wq.shape[1], 'gelu' if name == 'mlp.fc1' else None)
+        block, stage = divmod(seen, 6)
+        name, dst = f'blocks.{block}.' + stages[stage][0], stages[stage][1]
+        if 'norm' in name:
+            x = buf[dst].cpu().double()
+            plan.run(i, i + 1)
+            codes = rows('fp8_q', 'fp8_s', E)
+            check_layernorm(x, vit.w(name + '.weight').cpu(), vit.w(name + '.bias').cpu(), *codes)
+        else:
+            r = buf[stages[stage][2]].cpu().double() if stages[stage][2] else 0.0
+            if entry == 'vp_linear_fp8':
+                codes = fp8.quantize_rows(buf['ao' if 'proj' in name else 'h'])
+            plan.run(i, i + 1)
+            wq, ws = weights[name]
+            want, mag = fp8_oracle(*codes, wq, ws, vit.w(name + '.bias').cpu())
+            want, mag = want + r, mag + (r.abs() if stages[stage][2] else 0.0)
+            if dst is None:
+                codes = rows('fp8_hq', 'fp8_hs', Hd)
+                check_rounded(want, mag, wq.shape[1], *codes, act='gelu')
+            else:
+                assert buf[dst].dtype == (torch.float32 if stages[stage][2] else torch.bfloat16)
+                close(buf[dst], want, mag, wq.shape[1], 'gelu' if 'fc1' in name else None)
         seen += 1
-    assert seen == 4 * TOY['depth'] and torch.equal(out, heat)
+    assert seen == 6 * TOY['depth'] and torch.equal(out, heat)
     # the same network: every operand is off by 3 % in the mean, which is some 5 % of a Linear's result; a wrong scale, a lost
     # residual or a skipped Linear is of the size of the maps themselves
     rel = relerr(heat, eng.infer(img))[0]
@@ -197,6 +210,6 @@ def test_a_routed_vit_evaluates_on_8_bit_products():
     img = O.synth_batch(3, seed=3)[0].cuda()
     heat = eng.infer(img, fp8=True, dataset_source=[0, 2, 1])
     names = [c[0] for c in eng.plans[('infer', 3, 'fp8')][0].calls]
-    assert names.count('vp_linear_fp8') == 3 * TOY['depth']
+    assert sum(n in ('vp_linear_fp8', 'vp_gemm_fp8') for n in names) == 3 * TOY['depth']
     assert relerr(heat, eng.infer(img, dataset_source=[0, 2, 1]))[0] < 0.25
     assert not torch.equal(heat, eng.infer(img, fp8=True, dataset_source=[0, 1, 1]))

@@ -15,7 +15,7 @@ LIB_PATH = os.environ.get('VITPOSE_HIP_LIB') or os.path.join(_HERE, 'lib', 'libv
 
 VP_EPI_BF16, VP_EPI_GELU, VP_EPI_RESID_F32, VP_EPI_DGELU = 0, 1, 2, 3
 VP_EPI_SPLITK_F32, VP_EPI_F32, VP_EPI_SCALE_RELU, VP_EPI_DRELU, VP_EPI_PAIR = 4, 5, 6, 7, 8
-VP_F32, VP_BF16 = 0, 1
+VP_F32, VP_BF16, VP_E4M3 = 0, 1, 2
 
 
 class GemmArgs(Structure):
@@ -59,7 +59,8 @@ class GroupedArgs(Structure):
 class Fp8Args(Structure):
     _fields_ = [('M', c_int), ('N', c_int), ('K', c_int), ('xq', c_void_p), ('ldx', c_long), ('xs', c_void_p),
                 ('wq', c_void_p), ('ldw', c_long), ('ws', c_void_p), ('bias', c_void_p), ('act', c_int),
-                ('out', c_void_p), ('ldo', c_long), ('out_dtype', c_int), ('resid', c_void_p), ('ldr', c_long)]
+                ('out', c_void_p), ('ldo', c_long), ('out_dtype', c_int), ('resid', c_void_p), ('ldr', c_long),
+                ('oscale', c_void_p)]
 
 
 class LnPartial(Structure):
@@ -142,6 +143,7 @@ SIGNATURES = {
     'vp_grouped_wgrad_slices': [c_int, c_int, c_int, c_int],     # host-side helper: no stream argument
     'vp_quantize_fp8_rows': [P, c_int, c_long, c_int, c_int, P, P, P],
     'vp_quantize_fp8_weight': [P, c_int, c_long, c_int, c_int, P, P, P],
+    'vp_layernorm_fp8': [P, P, P, c_float, c_int, c_int, P, P, P],
     'vp_gemm_fp8': [POINTER(Fp8Args), P],
     'vp_linear_fp8': [POINTER(Fp8Args), P, c_int, c_long, c_int, P, P, P],
     'vp_linear_fp8_fused': [c_int, c_int, c_int, c_int],             # host-side helper: no stream argument

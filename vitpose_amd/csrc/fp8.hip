@@ -80,6 +80,72 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
     }
 }
 
+// ---- rows behind a LayerNorm: a wave holds a row, four blocks of it at a time, and the LayerNorm's weights ----
+template <int NB>
+__global__ __launch_bounds__(256) void layernorm_rows_kernel(const float* __restrict__ x, const float* __restrict__ gamma,
+                                                             const float* __restrict__ beta, float eps, int M, int E, int KB,
+                                                             uint8_t* __restrict__ q, float* __restrict__ scale) {
+    const int lane = threadIdx.x & 63, wave = blockIdx.x * 4 + (threadIdx.x >> 6), waves = gridDim.x * 4;
+    const int k0 = (lane >> 4) * BLK + (lane & 15) * 8;
+    float ga[NB][8], be[NB][8], v[NB][8], next[NB][8];
+    auto fetch = [&](long row) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (k0 + b * 512 < E) load8(x + row * E + k0 + b * 512, next[b]);
+    };
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ga[b][i] = be[b][i] = next[b][i] = 0.f;
+        if (k0 + b * 512 < E) {
+            load8(gamma + k0 + b * 512, ga[b]);
+            load8(beta + k0 + b * 512, be[b]);
+        }
+    }
+    const float n = 1.0f / (float)E;
+    if (wave < M) fetch(wave);
+    for (long row = wave; row < M; row += waves) {
+        float sum = 0.f, sq = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) { v[b][i] = next[b][i]; sum += v[b][i]; }
+        if (row + waves < M) fetch(row + waves);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o, 64);
+        const float mean = sum * n;
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+            if (k0 + b * 512 < E)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) { v[b][i] -= mean; sq += v[b][i] * v[b][i]; }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) sq += __shfl_xor(sq, o, 64);
+        const float rstd = rsqrtf(sq * n + eps);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[b][i] = v[b][i] * rstd * ga[b][i] + be[b][i];         // (zeros behind the row's end)
+                m = max(m, abs_bits(v[b][i]));
+            }
+#pragma unroll
+            for (int o = 1; o < 16; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+            float s, inv;
+            block_scale(m, s, inv);
+            const int kb = b * 4 + (lane >> 4);
+            if (kb < KB) {
+                uint2 out;
+                out.x = pack_e4m3(v[b][0] * inv, v[b][1] * inv, v[b][2] * inv, v[b][3] * inv);
+                out.y = pack_e4m3(v[b][4] * inv, v[b][5] * inv, v[b][6] * inv, v[b][7] * inv);
+                *reinterpret_cast<uint2*>(q + row * ((long)KB * BLK) + k0 + b * 512) = out;
+                if ((lane & 15) == 0) scale[(long)kb * M + row] = s;
+            }
+        }
+    }
+}
+
 // ---- weights: one workgroup per 128 x 128 square, 64 values a thread in registers between the two halves ----
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_weight_kernel(const T* __restrict__ w, long ldw, int N, int K, int KB,
@@ -127,6 +193,7 @@ struct Args {
     int act, out_f32;
     void* out; long ldo;
     const float* resid; long ldr;
+    float* oscale;                                            // not NULL: `out` is codes, these are their scales
 };
 
 __device__ __forceinline__ void dma16(const void* src, char* lds) {
@@ -154,18 +221,22 @@ __device__ __forceinline__ f32x4 gelu_f32(f32x4 v) {
     return v;
 }
 
-// one row's four columns j .. j + 3 (only those below N)
+// four columns j .. j + 3 of a row of the residual (only those below N)
+__device__ __forceinline__ f32x4 load_resid(const Args& a, long row, int j) {
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    const float* p = a.resid + row * a.ldr + j;
+    if (j + 3 < a.N && (a.ldr & 3) == 0) v = *reinterpret_cast<const f32x4*>(p);
+    else
+        for (int r = 0; r < 4; ++r)
+            if (j + r < a.N) v[r] = p[r];
+    return v;
+}
+
+// and of the result
 __device__ __forceinline__ void store4(const Args& a, long row, int j, f32x4 v) {
-    const bool whole = j + 3 < a.N && ((a.ldo | a.ldr) & 3) == 0;
+    const bool whole = j + 3 < a.N && (a.ldo & 3) == 0;
     if (a.out_f32) {
         float* o = (float*)a.out + row * a.ldo + j;
-        if (a.resid) {                                        // (read before its place in `out`, which may be the same, is written)
-            const float* p = a.resid + row * a.ldr + j;
-            if (whole) v += *reinterpret_cast<const f32x4*>(p);
-            else
-                for (int r = 0; r < 4; ++r)
-                    if (j + r < a.N) v[r] += p[r];
-        }
         if (whole) *reinterpret_cast<f32x4*>(o) = v;
         else
             for (int r = 0; r < 4; ++r)
@@ -199,7 +270,8 @@ __device__ __forceinline__ f32x4 load_bias(const Args& a, int j) {
 // are in flight (with none, the 256 x 256 tile waits for every burst of loads: 2 us a K tile for 0.9 of matrix instructions).
 // A lane's accumulators are in f32 units; a K tile's product starts from zero and is added with its block's scale (one FMA
 // a value: half of the matrix instructions' time, on another unit).
-template <int BM, int BN, int WN, int RING>
+// OUT: what is stored (the dtype tag): one kernel each, or the registers of one epilogue are spilled in another.
+template <int BM, int BN, int WN, int RING, int OUT>
 __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
 #ifdef __HIP_DEVICE_COMPILE__   // (the host pass has no buffer resources)
     constexpr int NT = 128 * WN, UX = BM / 64, UY = BN / 64, U = UX + UY, FM = BM / 32, FN = BN / WN / 16;
@@ -310,7 +382,53 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
     const int jw = j0 + wn * FN * 16, iw = i0 + wm * FM * 16;
 #pragma unroll
     for (int n = 0; n < FN; ++n) bias[n] = load_bias(a, jw + n * 16 + g * 4);
-    if (!a.out_f32 && ((a.N | (int)a.ldo) & 7) == 0) {
+    if constexpr (OUT == VP_E4M3) {
+        // The result as codes: a block of a row lies in PW waves, which meet at its largest magnitude in LDS.
+        constexpr int PW = BLK / (FN * 16), ROWS = FM * 16, CPITCH = FN * 16 + 16, SEG = FN;
+        static_assert(2 * WN * ROWS * 4 + 2 * WN * 16 * CPITCH <= RING * UNIT, "maxima and patches");
+        uint32_t* top = (uint32_t*)lds;
+        char* patch = lds + 2 * WN * ROWS * 4 + wave * 16 * CPITCH;
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int n = 0; n < FN; ++n) {
+                acc[m][n] = finish(a, acc[m][n], bias[n]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    if (jw + n * 16 + g * 4 + r >= a.N) acc[m][n][r] = 0.f;     // (columns behind the end: padding)
+                    most = max(most, abs_bits(acc[m][n][r]));
+                }
+            }
+            most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
+            most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
+            if (g == 0) top[wave * ROWS + m * 16 + li] = most;
+        }
+        __syncthreads();
+        const int jb = jw / BLK;
+        const bool inside = jb * BLK < a.N;
+#pragma unroll
+        for (int m = 0; m < FM; ++m) {
+            uint32_t most = 0;
+#pragma unroll
+            for (int p = 0; p < PW; ++p) most = max(most, top[(wave - wn % PW + p) * ROWS + m * 16 + li]);
+            float scale, inv;
+            block_scale(most, scale, inv);
+            const int row = iw + m * 16 + li;
+            if (inside && wn % PW == 0 && g == 0 && row < a.M) a.oscale[(long)jb * a.M + row] = scale;
+#pragma unroll
+            for (int n = 0; n < FN; ++n)
+                *reinterpret_cast<uint32_t*>(patch + li * CPITCH + n * 16 + g * 4) =
+                    pack_e4m3(acc[m][n][0] * inv, acc[m][n][1] * inv, acc[m][n][2] * inv, acc[m][n][3] * inv);
+            if (lane < 16 * SEG) {
+                const int r = lane / SEG, c16 = lane % SEG * 16, i = iw + m * 16 + r;
+                const i32x4 v = *reinterpret_cast<const i32x4*>(patch + r * CPITCH + c16);
+                if (inside && i < a.M) *reinterpret_cast<i32x4*>((uint8_t*)a.out + i * a.ldo + jw + c16) = v;
+            }
+        }
+        return;
+    }
+    if (OUT == VP_BF16 && ((a.N | (int)a.ldo) & 7) == 0) {
         // through a patch of LDS of the wave's own, sixteen rows at a time, so that a lane stores sixteen bytes of a row
         constexpr int SEG = FN * 2;
         char* patch = lds + wave * 16 * PITCH;
@@ -330,15 +448,30 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
         }
         return;
     }
-#pragma unroll
-    for (int m = 0; m < FM; ++m) {
-        const int i = iw + m * 16 + li;
-        if (i >= a.M) continue;
+    // four rows of the residual are on their way before the first is added
+    constexpr int AHEAD = FM < 4 ? FM : 4;
+    f32x4 res[AHEAD][FN];
+    auto fetch = [&](int m) {
 #pragma unroll
         for (int n = 0; n < FN; ++n) {
             const int j = jw + n * 16 + g * 4;
-            if (j < a.N) store4(a, i, j, finish(a, acc[m][n], bias[n]));
+            res[m % AHEAD][n] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (OUT == VP_F32 && a.resid && j < a.N) res[m % AHEAD][n] = load_resid(a, min(iw + m * 16 + li, a.M - 1), j);
         }
+    };
+#pragma unroll
+    for (int m = 0; m < AHEAD; ++m) fetch(m);
+#pragma unroll
+    for (int m = 0; m < FM; ++m) {
+        const int i = iw + m * 16 + li;
+#pragma unroll
+        for (int n = 0; n < FN; ++n) {
+            const int j = jw + n * 16 + g * 4;
+            f32x4 v = finish(a, acc[m][n], bias[n]);
+            if (OUT == VP_F32 && a.resid) v += res[m % AHEAD][n];
+            if (i < a.M && j < a.N) store4(a, i, j, v);
+        }
+        if (m + AHEAD < FM) fetch(m + AHEAD);
     }
 #endif
 }
@@ -435,7 +568,9 @@ __global__ __launch_bounds__(512, 2) void fp8_narrow_kernel(Args a, const T* __r
         f32x4 v = *reinterpret_cast<const f32x4*>(&part[0][r][c]);
 #pragma unroll
         for (int w = 1; w < 8; ++w) v += *reinterpret_cast<const f32x4*>(&part[w][r][c]);
-        store4(a, i, j, finish(a, v, load_bias(a, j)));
+        v = finish(a, v, load_bias(a, j));
+        if (a.resid) v += load_resid(a, i, j);
+        store4(a, i, j, v);
     }
 }
 
@@ -461,6 +596,18 @@ extern "C" int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, i
     VP_LAUNCH_RET();
 }
 
+extern "C" int vp_layernorm_fp8(const float* x, const float* gamma, const float* beta, float eps, int M, int E, void* q,
+                                float* scale, hipStream_t stream) {
+    VP_CHECK_ARG(M >= 0 && M <= 1 << 29 && E >= 8 && E % 8 == 0 && E <= 2048);
+    if (M == 0) return VP_OK;
+    VP_CHECK_ARG(x && gamma && beta && q && scale && aligned16(x) && aligned16(gamma) && aligned16(beta) && aligned16(q));
+    const int KB = cdiv(E, BLK), grid = std::min(cdiv(M, 4), 2048);
+    auto kernel = E <= 512 ? layernorm_rows_kernel<1> : E <= 1024 ? layernorm_rows_kernel<2>
+                : E <= 1536 ? layernorm_rows_kernel<3> : layernorm_rows_kernel<4>;
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), 0, stream, x, gamma, beta, eps, M, E, KB, (uint8_t*)q, scale);
+    VP_LAUNCH_RET();
+}
+
 extern "C" int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale,
                                       hipStream_t stream) {
     VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && N >= 1 && K >= 8 && K % 8 == 0 && ldw >= K && ldw % 8 == 0);
@@ -481,17 +628,18 @@ namespace {
 
 int check_fp8(const vp_fp8_args* g) {
     VP_CHECK_ARG(g && g->M >= 0 && g->M <= 1 << 29 && g->N >= 1 && g->K >= BLK && g->K % BLK == 0 && (g->act == 0 || g->act == 1));
-    VP_CHECK_ARG(g->out_dtype == VP_F32 || g->out_dtype == VP_BF16);
+    VP_CHECK_ARG(g->out_dtype == VP_F32 || g->out_dtype == VP_BF16 || g->out_dtype == VP_E4M3);
     if (g->M == 0) return VP_OK;
     VP_CHECK_ARG(g->wq && g->ws && g->out && aligned16(g->wq) && aligned16(g->out));
     VP_CHECK_ARG(g->ldw >= g->K && g->ldo >= g->N && g->ldw % 16 == 0);
+    VP_CHECK_ARG(g->out_dtype != VP_E4M3 || (g->oscale && g->ldo % 16 == 0 && g->ldo >= (long)cdiv(g->N, BLK) * BLK));
     VP_CHECK_ARG(!g->resid || (g->out_dtype == VP_F32 && g->ldr >= g->N && aligned16(g->resid)));
     return VP_OK;
 }
 
 Args make_args(const vp_fp8_args* g) {
     return Args{g->M, g->N, g->K / BLK, (const uint8_t*)g->xq, g->ldx, g->xs, (const uint8_t*)g->wq, g->ldw, g->ws, g->bias,
-                g->act, g->out_dtype == VP_F32, g->out, g->ldo, g->resid, g->resid ? g->ldr : 0};
+                g->act, g->out_dtype == VP_F32, g->out, g->ldo, g->resid, g->ldr, g->out_dtype == VP_E4M3 ? g->oscale : nullptr};
 }
 
 template <typename T, int FM, int FN>
@@ -537,14 +685,19 @@ int best_narrow(int M, int N, double row_weight, double& cost) {
     return best;
 }
 
-int product_kernel(int M, int N, double& cost) {
-    const int s = best_narrow(M, N, 1.0, cost);
+int tile_kernel(int M, int N, double& cost) {
     const double w128 = std::max(1.0, (double)cdiv(M, 128) * cdiv(N, 128) / 256);
     const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
-    const double tile = 205 * std::min(w128, 2.75 * w256);
+    cost = 205 * std::min(w128, 2.75 * w256);
+    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
+}
+
+int product_kernel(int M, int N, double& cost) {
+    double tile;
+    const int s = best_narrow(M, N, 1.0, cost), t = tile_kernel(M, N, tile);
     if (cost <= tile) return s;
     cost = tile;
-    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
+    return t;
 }
 
 // The few-rows kernel that rounds its rows itself, or -1: a launch of the quantizer costs about 4 us more, a unit of the costs above
@@ -561,7 +714,9 @@ int launch_tile(const vp_fp8_args* g, hipStream_t stream) {
     const int tn = cdiv(g->N, BN);
     const long grid = (long)cdiv(g->M, BM) * tn;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
-    hipLaunchKernelGGL((fp8_kernel<BM, BN, WN, RING>), dim3((unsigned)grid), dim3(128 * WN), 0, stream, make_args(g), tn);
+    auto kernel = g->out_dtype == VP_F32 ? fp8_kernel<BM, BN, WN, RING, VP_F32>
+                : g->out_dtype == VP_BF16 ? fp8_kernel<BM, BN, WN, RING, VP_BF16> : fp8_kernel<BM, BN, WN, RING, VP_E4M3>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(128 * WN), 0, stream, make_args(g), tn);
     VP_LAUNCH_RET();
 }
 
@@ -573,7 +728,7 @@ extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
     VP_CHECK_ARG(g->xq && g->xs && aligned16(g->xq) && g->ldx >= g->K && g->ldx % 16 == 0);
     VP_CHECK_ARG(g->ldx <= 1 << 22 && g->ldw <= 1 << 22);       // a tile's rows within 32-bit offsets
     double cost;
-    const int which = product_kernel(g->M, g->N, cost);
+    const int which = g->out_dtype == VP_E4M3 ? tile_kernel(g->M, g->N, cost) : product_kernel(g->M, g->N, cost);
     if (which < TILE_128) return launch_narrow<uint8_t>(which, g, (const uint8_t*)g->xq, g->ldx, g->K, stream);
     if (which == TILE_256) return launch_tile<256, 256, 4, 18>(g, stream);
     // one workgroup a CU: eight waves; two: four waves each (3000 x 2000 x 3000: 31 us against 34; 192 x 4096 x 1024: 8.5 / 8.1)
@@ -589,7 +744,7 @@ extern "C" int vp_linear_fp8(const vp_fp8_args* g, const void* x, int dtype, lon
                              hipStream_t stream) {
     if (int rc = check_fp8(g)) return rc;
     VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && K >= 8 && K % 8 == 0 && cdiv(K, BLK) * BLK == g->K);
-    VP_CHECK_ARG(ldx >= K && ldx % 8 == 0);
+    VP_CHECK_ARG(ldx >= K && ldx % 8 == 0 && g->out_dtype != VP_E4M3);
     if (g->M == 0) return VP_OK;
     VP_CHECK_ARG(x && aligned16(x));
     const int shape = fused_kernel(g->M, g->N, K, dtype);

@@ -478,38 +478,52 @@ class VitRunner:
     def record_forward_fp8(self, plan: Plan, ws: Workspace, img: torch.Tensor, B: int,
                            tokens_f32: Optional[torch.Tensor] = None):
         """Evaluation forward with the Blocks' Linears (vit.py:66-74,93,96) as products of e4m3 operands, one f32 scale per
-        row and 128 values of the activations and per 128 x 128 square of a weight.  The patch embedding, attention, the
-        LayerNorms and the residual stream stay what they are in record_forward."""
+        row and 128 values of the activations and per 128 x 128 square of a weight.  norm1 / norm2 emit the codes that qkv
+        and fc1 read, fc1 those that fc2 reads; attention, the patch embedding and the residual stream stay what they are in
+        record_forward."""
         E, T, M, Hd = self.E, self.T, B * self.T, self.hidden
         H, W = self.img_hw
         weights = self._fp8_buffers()[0]
-        kmax = (max(E, Hd) + 127) // 128
-        xq, xs = ws.get('fp8_q', (M * kmax * 128,), torch.uint8), ws.f32('fp8_s', M * kmax)
+        kbE, kbH = (E + 127) // 128, (Hd + 127) // 128
+        xq, xs = ws.get('fp8_q', (M * max(kbE, kbH) * 128,), torch.uint8), ws.f32('fp8_s', M * max(kbE, kbH))
+        hq, hs = ws.get('fp8_hq', (M * kbH * 128,), torch.uint8), ws.f32('fp8_hs', M * kbH)
+        # fc1 hands codes to fc2 where fc2 takes codes: few rows are rounded by fc2's own kernel instead
+        to_codes = not self.part and not plan.L.vp_linear_fp8_fused(M, E, Hd, _lib.VP_BF16)
 
-        def linear(name, x, out, N, K, **more):
-            bias = self.w(name + '.bias') if self.has(name + '.bias') else None
-            plan.linear_fp8(x, *weights[name], out, M, N, K, xq, xs, bias=bias, **more)
+        def weight(name):
+            return weights[name] + (self.w(name + '.bias') if self.has(name + '.bias') else None,)
+
+        def norm(name, x):
+            plan.layernorm_fp8(x, self.w(name + '.weight'), self.w(name + '.bias'), xq, xs, M, E)
 
         col = ws.bf16('pe_col', M, self.Kpe)
         plan.patch_im2col(img, col, B, self.C, H, W, self.patch, self.stride, self.pad)
         x, xm = ws.f32('x_a', M, E), ws.f32('x_b', M, E)
         plan.gemm(col, self.h('patch_embed.proj.weight'), x, M, E, self.Kpe, ldx=self.Kpe, ldy=self.Kpe, ldo=E,
                   epilogue=_lib.VP_EPI_RESID_F32, bias=self.w('patch_embed.proj.bias'), pos=self.pos_comb, pos_rows=T)
-        xn, qkv = ws.bf16('xn1', M, E), ws.bf16('qkv', M, 3 * E)
-        ao, hact = ws.bf16('ao', M, E), ws.bf16('h', M, Hd)
+        qkv, ao, hact = ws.bf16('qkv', M, 3 * E), ws.bf16('ao', M, E), ws.bf16('h', M, Hd)
         for i in range(self.depth):
             b = f'blocks.{i}.'
-            plan.layernorm_fwd(x, self.w(b + 'norm1.weight'), self.w(b + 'norm1.bias'), xn, None, None, None, M, E)
-            linear(b + 'attn.qkv', xn, qkv, 3 * E, E)
+            norm(b + 'norm1', x)
+            wq, sc, bias = weight(b + 'attn.qkv')
+            plan.gemm_fp8(xq, xs, wq, sc, qkv, M, 3 * E, E, bias=bias)
             plan.attention_fwd(qkv, ao, None, B, self.heads, self.d, T, self.scale)
-            linear(b + 'attn.proj', ao, xm, E, E, resid=x)
-            plan.layernorm_fwd(xm, self.w(b + 'norm2.weight'), self.w(b + 'norm2.bias'), xn, None, None, None, M, E)
-            linear(b + 'mlp.fc1', xn, hact, Hd, E, gelu=True)
+            wq, sc, bias = weight(b + 'attn.proj')
+            plan.linear_fp8(ao, wq, sc, xm, M, E, E, xq, xs, bias=bias, resid=x)
+            norm(b + 'norm2', xm)
+            wq, sc, bias = weight(b + 'mlp.fc1')
+            if to_codes:
+                plan.gemm_fp8(xq, xs, wq, sc, hq, M, Hd, E, bias=bias, gelu=True, oscale=hs)
+                wq, sc, bias = weight(b + 'mlp.fc2')
+                plan.gemm_fp8(hq, hs, wq, sc, x, M, E, Hd, bias=bias, resid=xm)
+                continue
+            plan.gemm_fp8(xq, xs, wq, sc, hact, M, Hd, E, bias=bias, gelu=True)
             if self.part:
                 plan.gemm(hact, self.h(b + 'mlp.fc2.weight'), x, M, E, Hd, ldx=Hd, ldy=Hd, ldo=E,
                           epilogue=_lib.VP_EPI_RESID_F32, bias=self.w(b + 'mlp.fc2.bias'), resid=xm, route=self._route(ws, B, i))
             else:
-                linear(b + 'mlp.fc2', hact, x, E, Hd, resid=xm)
+                wq, sc, bias = weight(b + 'mlp.fc2')
+                plan.linear_fp8(hact, wq, sc, x, M, E, Hd, xq, xs, bias=bias, resid=xm)
         feat = ws.bf16('feat', M, E)
         if self.cfg.get('last_norm', True):
             plan.layernorm_fwd(x, self.w('last_norm.weight'), self.w('last_norm.bias'), feat, tokens_f32, None, None, M, E)

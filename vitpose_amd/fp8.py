@@ -9,6 +9,9 @@ or, where several products read the same rows,
     xq, xs = quantize_rows(x)                              # e4m3 [M, Kp], scales [Kp / 128, M]
     y = product(xq, xs, wq, ws, bias)
 
+`layernorm_rows` gives the rows behind a LayerNorm in that form, and a product with out_dtype = torch.float8_e4m3fn its
+result: what lies between two products then never exists in 16 bits.
+
 Kp is K rounded up to 128.  Nothing here synchronises.
 """
 import ctypes
@@ -16,7 +19,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import VP_BF16, VP_F32, Fp8Args
+from ._lib import VP_BF16, VP_E4M3, VP_F32, Fp8Args
 
 BLOCK = 128
 _F8, _BF16, _F32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
@@ -103,6 +106,26 @@ def quantize_weight(w):
     return q, scale
 
 
+def layernorm_rows(x, weight, bias, eps=1e-6):
+    """quantize_rows of the LayerNorm of x f32 [M, E] over its rows (E a multiple of 8, at most 2048)."""
+    tag, ld = _real_matrix(x, 'x')
+    M, E = x.shape
+    if tag != VP_F32:
+        raise TypeError('x: expected float32 (the residual stream)')
+    if ld != E or E > 2048:
+        raise ValueError(f'x: shape {tuple(x.shape)}, strides {x.stride()}: contiguous rows of at most 2048 values')
+    for t, what in ((weight, 'weight'), (bias, 'bias')):
+        _vector(t, what, (E,), x.device)
+        if t.data_ptr() % 16:
+            raise ValueError(f'{what}: must start on a 16-byte boundary')
+    kb = (E + BLOCK - 1) // BLOCK
+    q = x.new_empty((M, kb * BLOCK), dtype=_F8)
+    scale = x.new_empty((kb, M))
+    if M:
+        _lib.launch(x.get_device(), 'vp_layernorm_fp8', x.data_ptr(), weight.data_ptr(), bias.data_ptr(), eps, M, E, q.data_ptr(), scale.data_ptr())
+    return q, scale
+
+
 def _result(M, N, out, out_dtype, like):
     """(result, its leading dimension, dtype tag)."""
     if out is None:
@@ -156,7 +179,8 @@ def _residual(resid, M, N, tag, dev):
 
 def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
     """act(xq wq^T with the blocks' scales + bias) (+ resid), bf16 or f32 [M, N]; operands as the quantizers return them.
-    resid (f32 results only) may be `out` itself."""
+    resid (f32 results only) may be `out` itself.  out_dtype = torch.float8_e4m3fn: (codes, scales) of the result, as
+    quantize_rows would return them, but from the sums in f32 (no out, no resid)."""
     try:
         d, p = xq.get_device(), xq.data_ptr()
         M, Kx = xq.shape
@@ -175,6 +199,16 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
     ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, xq.device)
     if Kx != Kp:
         raise ValueError(f'xq {tuple(xq.shape)} against wq {tuple(wq.shape)}: Kp differs')
+    if out_dtype is _F8:
+        if out is not None or resid is not None:
+            raise ValueError('out_dtype float8_e4m3fn takes neither out nor resid')
+        nb = (N + 127) // BLOCK
+        q, s = xs.new_empty((M, nb * BLOCK), dtype=_F8), xs.new_empty((nb, M))
+        if M:
+            args = Fp8Args(M, N, Kp, p, ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], q.data_ptr(), nb * BLOCK,
+                           VP_E4M3, None, 0, s.data_ptr())
+            _lib.launch(d, _lib.lib().vp_gemm_fp8, ctypes.byref(args))
+        return q, s
     out, ldo, tag = _result(M, N, out, out_dtype, xs)
     pr, ldr = _residual(resid, M, N, tag, xq.device) if resid is not None else (None, 0)
     if M and N:
@@ -187,6 +221,8 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
 def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
     """act(x w^T + bias) (+ resid) with x rounded to e4m3 on the way: `quantize_rows` and `product` in one call (one launch where the
     rows are few; the blocks of K may then be added up in another order)."""
+    if out_dtype is _F8:
+        return product(*quantize_rows(x), wq, ws, bias, act, out_dtype, out, resid)
     d, p, tag, ldx = _rows(x)
     M, K = x.shape
     ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, x.device)

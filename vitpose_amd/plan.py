@@ -496,15 +496,35 @@ class Plan:
     def linear_fp8(self, x, wq, ws, out, M, N, K, xq, xs, bias=None, gelu=False, resid=None):
         """out (bf16, or f32 with an optional f32 resid) [M][N] = x w^T + bias, x bf16 [M][K] rounded to e4m3 on the way;
         xq (uint8, M * Kp) and xs (f32, M * Kp / 128): scratch."""
-        _chk(x, torch.bfloat16, 'x'), _chk(xq, torch.uint8, 'xq'), _chk(xs, torch.float32, 'xs')
-        kb = (K + 127) // 128
-        assert x.numel() >= M * K and out.numel() >= M * N and xq.numel() >= M * kb * 128 and xs.numel() >= M * kb
-        assert wq.dtype == torch.float8_e4m3fn and wq.numel() >= N * kb * 128 and ws.numel() >= (N + 127) // 128 * kb
-        assert resid is None or (out.dtype == resid.dtype == torch.float32 and resid.numel() >= M * N)
-        args = _lib.Fp8Args(M, N, kb * 128, None, 0, None, _p(wq), kb * 128, _p(ws), _p(bias), int(gelu), _p(out), N,
-                            _lib.VP_F32 if out.dtype == torch.float32 else _lib.VP_BF16, _p(resid), N)
+        _chk(x, torch.bfloat16, 'x')
+        assert x.numel() >= M * K
+        args = self._fp8_args(wq, ws, out, M, N, K, xq, xs, bias, gelu, resid, None)
         self._add('vp_linear_fp8', ctypes.byref(args), _p(x), _lib.VP_BF16, K, K, _p(xq), _p(xs),
                   keep=(args, x, wq, ws, out, xq, xs, bias, resid))
+
+    def gemm_fp8(self, xq, xs, wq, ws, out, M, N, K, bias=None, gelu=False, resid=None, oscale=None):
+        """The same of rows that are codes xq (uint8) and scales xs already; with oscale, out (uint8) and oscale become the
+        result's."""
+        args = self._fp8_args(wq, ws, out, M, N, K, xq, xs, bias, gelu, resid, oscale)
+        args.xq, args.ldx, args.xs = _p(xq), args.K, _p(xs)
+        self._add('vp_gemm_fp8', ctypes.byref(args), keep=(args, xq, xs, wq, ws, out, bias, resid, oscale))
+
+    def _fp8_args(self, wq, ws, out, M, N, K, xq, xs, bias, gelu, resid, oscale):
+        _chk(xq, torch.uint8, 'xq'), _chk(xs, torch.float32, 'xs'), _chk(wq, torch.float8_e4m3fn, 'wq'), _chk(ws, torch.float32, 'ws')
+        kb, nb = (K + 127) // 128, (N + 127) // 128
+        ldo = nb * 128 if oscale is not None else N
+        assert xq.numel() >= M * kb * 128 and xs.numel() >= M * kb and wq.numel() >= N * kb * 128 and ws.numel() >= nb * kb
+        assert out.numel() >= M * ldo and (oscale is None or (out.dtype == torch.uint8 and oscale.numel() >= M * nb and resid is None))
+        assert resid is None or (out.dtype == resid.dtype == torch.float32 and resid.numel() >= M * N)
+        tag = {torch.float32: _lib.VP_F32, torch.bfloat16: _lib.VP_BF16, torch.uint8: _lib.VP_E4M3}[out.dtype]
+        return _lib.Fp8Args(M, N, kb * 128, None, 0, None, _p(wq), kb * 128, _p(ws), _p(bias), int(gelu), _p(out), ldo, tag,
+                            _p(resid), N, _p(oscale))
+
+    def layernorm_fp8(self, x, gamma, beta, xq, xs, M, E, eps=1e-6):
+        _chk(x, torch.float32, 'x'), _chk(xq, torch.uint8, 'xq'), _chk(xs, torch.float32, 'xs')
+        kb = (E + 127) // 128
+        assert x.numel() >= M * E and xq.numel() >= M * kb * 128 and xs.numel() >= M * kb
+        self._add('vp_layernorm_fp8', _p(x), _p(gamma), _p(beta), eps, M, E, _p(xq), _p(xs), keep=(x, gamma, beta, xq, xs))
 
     # -- fp32-accurate path (hi / lo pair arrays; the products are gemm(..., split3=True)) --
     def split_pair(self, x, pair, n):
