@@ -354,7 +354,7 @@ int vp_wgrad_grouped_kmap_bf16(const vp_group_entry* table_dev, int count, int t
  *   The products take such a list, or rows = NULL: entry i of the list is then row i.  Entries outside [0, T) are left
  *     out, offsets are cut to [0, T]; no row may be listed twice.  bf16 operands, sums in f32, each result rounded once.
  *     x [T][ldx >= K], w [E][N][ldw >= K] (experts stride_w apart), dy [T][ldy >= N], bias [E][N] f32 (stride_b apart).
- *     N, K and every leading dimension multiples of 8, pointers on 16 bytes.
+ *     N, K and every leading dimension multiples of 8, pointers on 16 bytes, T at most 2^30.
  *     fwd:   out [T][ldo >= N] bf16 = x w^T + bias
  *     dgrad: out [T][ldo >= K] bf16 = dy w
  *     wgrad: dw [E][N][K] f32 = dy^T x, db [E][N] f32 (optional) = column sums of dy; zeros for an expert without rows.

@@ -326,3 +326,22 @@ def test_refusals():
     for n in (0, 513):
         with pytest.raises(ValueError):
             experts.expert_rows(rows, n)
+
+
+def test_a_gradient_off_its_sixteen_bytes_and_a_layer_without_bias():
+    """autograd may hand over any contiguous view; a layer whose input needs no gradient still gets its weights'."""
+    g = torch.Generator().manual_seed(3)
+    layer = experts.ExpertLinear(3, 16, 8, bias=False, device='cuda')
+    x = torch.randn(5, 16, generator=g).bfloat16().cuda()
+    e = torch.tensor([2, 0, 2, 1, -1], dtype=torch.int32).cuda()
+    flat = torch.randn(5 * 8 + 1, generator=g).bfloat16().cuda()
+    dy = flat[1:].view(5, 8)
+    assert dy.data_ptr() % 16
+    y = layer(x, e)
+    y.backward(dy)
+    want = torch.zeros(3, 8, 16, dtype=torch.float64)
+    for t, k in enumerate(e.tolist()):
+        if k >= 0:
+            want[k] += dy[t].cpu().double()[:, None] * x[t].cpu().double()
+    # two products of bf16 numbers at most are added in f32
+    assert (layer.weight.grad.cpu().double() - want).abs().max() <= 4 * 2.0 ** -24 * 16

@@ -231,3 +231,20 @@ def test_every_entry_is_called_with_the_header_s_arguments():
                 assert ctypes.sizeof(t) == ctypes.sizeof(ctypes.c_void_p), f'{name}: {p}'
         checked += 1
     assert checked > 40
+
+
+@pytest.mark.parametrize('eps,rc', [(0.0, 0), (1e-8, 0), (1.2e-38, 0), (1e-40, ERR_ARG), (float('nan'), ERR_ARG)])
+def test_adamw8_takes_no_eps_that_the_division_flushes(eps, rc):
+    # (an empty table: nothing is launched, only the arguments are looked at)
+    assert adamw8(eps=eps, nchunks=0) == rc
+
+
+def test_row_counts_beyond_32_bit_arithmetic_are_refused():
+    import ctypes
+    from vitpose_amd._lib import GroupedArgs
+    L, T = _lib.lib(), (1 << 30) + 1
+    assert L.vp_expert_rows(64, T, 4, 64, 64, None) == ERR_ARG
+    a = GroupedArgs(T, 4, 64, 64, 64, 64, 64, 64, 64, 64, 64 * 64, None, 0, 64, 64, 64, 64, 0)
+    assert L.vp_grouped_fwd(ctypes.byref(a), None) == ERR_ARG
+    assert L.vp_grouped_dgrad(ctypes.byref(a), None) == ERR_ARG
+    assert L.vp_grouped_wgrad(ctypes.byref(a), 64, None, None, 0, None) == ERR_ARG

@@ -173,6 +173,11 @@ def test_a_vit_trained_with_8_bit_moments_evaluates_on_8_bit_products(B):
     with pytest.raises(ValueError):
         eng.infer(img, fp8=True, fold_ln=True)
     assert eng.infer(img[:1], fp8=True).shape[0] == 1
+    # an engine set to 8 bits still takes another path where a call names it
+    eng.fp8 = True
+    want = [eng.infer(img, fp8=False, fold_ln=True), eng.infer(img, fp8=False), eng.infer(img, fp8=False, exact=True)]
+    assert torch.equal(eng.infer(img, fold_ln=True), want[0]) and torch.equal(eng.infer(img, exact=True), want[2])
+    assert torch.equal(eng.infer(img), heat) and not torch.equal(heat, want[1])
 
 
 def test_test_cfg_chooses_8_bit_products_and_refuses_two_paths_at_once():

@@ -841,12 +841,14 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int
     }
 }
 
+constexpr int MAX_T = 1 << 30;                         // row numbers, and a tile or a run behind them, stay in 32 bits
+
 int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
 }  // namespace
 
 extern "C" int vp_expert_rows(const int* expert, int T, int E, int* rows, int* offsets, hipStream_t stream) {
-    VP_CHECK_ARG(T >= 0 && E >= 1 && offsets && (T == 0 || (expert && rows)));
+    VP_CHECK_ARG(T >= 0 && T <= MAX_T && E >= 1 && offsets && (T == 0 || (expert && rows)));
     if (E > SORT_MAX_E) return VP_ERR_UNSUPPORTED;
     if (E <= FEW_E) {
         hipLaunchKernelGGL(expert_rows_few_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, expert, T, E, rows, offsets);
@@ -861,7 +863,7 @@ extern "C" int vp_expert_rows(const int* expert, int T, int E, int* rows, int* o
 namespace {
 
 int check_common(const vp_grouped_args* g) {
-    VP_CHECK_ARG(g && g->T >= 0 && g->E >= 1 && g->N >= 8 && g->K >= 8 && g->N % 8 == 0 && g->K % 8 == 0 && g->offsets);
+    VP_CHECK_ARG(g && g->T >= 0 && g->T <= MAX_T && g->E >= 1 && g->N >= 8 && g->K >= 8 && g->N % 8 == 0 && g->K % 8 == 0 && g->offsets);
     return VP_OK;
 }
 
@@ -952,9 +954,8 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // The kernels differ in how many bytes a CU has to fetch: a workgroup reads tile rows + tile columns operand rows, 256 run
     // at a time, and a CU takes in some 50 KB a microsecond, whoever else is running -- twice that where the loads go to LDS
     // four K tiles ahead, as in the 128 x 128 kernel.  The smallest (rounds x operand rows) wins; it ranks what was measured
-    // right.  K 4096, N 256, 6 experts, us at 1 / 192 / 768 / 1536 / 3072 rows: 16 x 16 7.1 / 17.9 / 31.5 / 52 / 94, 16 x 32
-    // 10.9 / 15.0 / 25 / 46 / 77, 32 x 32 12.2 / 18.6 / 18.9 / 34 / 65, 32 x 64 19.0 / 25.4 / 25.4 / 25.8 / 49, 128 x 128
-    // 31.1 / 32.0 / 32.4 / 32.5 / 33.  K 1024, N 1024, 24 experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 /
+    // right.  K 4096, N 256, 6 experts, us at 1 / 192 / 768 / 1536 rows: 16 x 16 7.1 / 17.9 / 31.5 / 52, 16 x 32 10.9 / 15.0 / 25 / 46,
+    // 32 x 32 12.2 / 18.6 / 18.9 / 34, 32 x 64 19.0 / 25.4 / 25.4 / 25.8, 128 x 128 31.1 / 32.0 / 32.4 / 32.5.  K 1024, N 1024, 24 experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 /
     // 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
     const auto cost = [&](int tm, int tn, int weight) {
         const long tiles = g->T / tm + (std::min(g->E, g->T) + 1) / 2;         // experts' last tiles: half full on average

@@ -685,19 +685,14 @@ int best_narrow(int M, int N, double row_weight, double& cost) {
     return best;
 }
 
-int tile_kernel(int M, int N, double& cost) {
+int product_kernel(int M, int N, double& cost) {
+    const int s = best_narrow(M, N, 1.0, cost);
     const double w128 = std::max(1.0, (double)cdiv(M, 128) * cdiv(N, 128) / 256);
     const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
-    cost = 205 * std::min(w128, 2.75 * w256);
-    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
-}
-
-int product_kernel(int M, int N, double& cost) {
-    double tile;
-    const int s = best_narrow(M, N, 1.0, cost), t = tile_kernel(M, N, tile);
+    const double tile = 205 * std::min(w128, 2.75 * w256);
     if (cost <= tile) return s;
     cost = tile;
-    return t;
+    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
 }
 
 // The few-rows kernel that rounds its rows itself, or -1: a launch of the quantizer costs about 4 us more, a unit of the costs above
@@ -714,8 +709,9 @@ int launch_tile(const vp_fp8_args* g, hipStream_t stream) {
     const int tn = cdiv(g->N, BN);
     const long grid = (long)cdiv(g->M, BM) * tn;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
-    auto kernel = g->out_dtype == VP_F32 ? fp8_kernel<BM, BN, WN, RING, VP_F32>
-                : g->out_dtype == VP_BF16 ? fp8_kernel<BM, BN, WN, RING, VP_BF16> : fp8_kernel<BM, BN, WN, RING, VP_E4M3>;
+    auto kernel = g->out_dtype == VP_F32 ? fp8_kernel<BM, BN, WN, RING, VP_F32> : fp8_kernel<BM, BN, WN, RING, VP_BF16>;
+    if constexpr (BN == BLK)
+        if (g->out_dtype == VP_E4M3) kernel = fp8_kernel<BM, BN, WN, RING, VP_E4M3>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(128 * WN), 0, stream, make_args(g), tn);
     VP_LAUNCH_RET();
 }
@@ -727,8 +723,11 @@ extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
     if (g->M == 0) return VP_OK;
     VP_CHECK_ARG(g->xq && g->xs && aligned16(g->xq) && g->ldx >= g->K && g->ldx % 16 == 0);
     VP_CHECK_ARG(g->ldx <= 1 << 22 && g->ldw <= 1 << 22);       // a tile's rows within 32-bit offsets
+    // Codes: 128 x 128 tiles, two of which share a CU: one's largest magnitudes, rounding and GELU, 20 us of a 256 x 256 tile, pass
+    // under the other's matrix instructions (6144 x 4096 x 1024: 52 us
+    // against 65; 24576 x 5120 x 1280: 277 against 301).
     double cost;
-    const int which = g->out_dtype == VP_E4M3 ? tile_kernel(g->M, g->N, cost) : product_kernel(g->M, g->N, cost);
+    const int which = g->out_dtype == VP_E4M3 ? TILE_128 : product_kernel(g->M, g->N, cost);
     if (which < TILE_128) return launch_narrow<uint8_t>(which, g, (const uint8_t*)g->xq, g->ldx, g->K, stream);
     if (which == TILE_256) return launch_tile<256, 256, 4, 18>(g, stream);
     // one workgroup a CU: eight waves; two: four waves each (3000 x 2000 x 3000: 31 us against 34; 192 x 4096 x 1024: 8.5 / 8.1)

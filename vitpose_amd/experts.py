@@ -8,7 +8,7 @@ row).
     dweight, dbias = grouped_linear_wgrad(dy, x, offsets, rows)     # f32 [E, N, K], [E, N]
 
 `ExpertLinear` is the module with f32 master parameters and autograd on top of them.  Operands are bf16, sums f32.  The
-routing stays on the device; nothing here synchronises.
+routing stays on the device; nothing here synchronises.  The functions do not record gradients, the module does.
 """
 import ctypes
 
@@ -199,6 +199,8 @@ class _GroupedLinear(torch.autograd.Function):
     def backward(ctx, dy):
         x, w, offsets, rows = ctx.saved_tensors
         dy = dy.contiguous()
+        if dy.data_ptr() % 16:
+            dy = dy.clone()
         dx = grouped_linear_dgrad(dy, w, offsets, rows) if ctx.needs_input_grad[0] else None
         dw = db = None
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:

@@ -12,7 +12,7 @@ or, where several products read the same rows,
 `layernorm_rows` gives the rows behind a LayerNorm in that form, and a product with out_dtype = torch.float8_e4m3fn its
 result: what lies between two products then never exists in 16 bits.
 
-Kp is K rounded up to 128.  Nothing here synchronises.
+Kp is K rounded up to 128.  Nothing here synchronises or records gradients.
 """
 import ctypes
 

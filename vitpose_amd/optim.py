@@ -123,8 +123,8 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
         plain = False
     if not plain:
         _check_adamw8(param, grad, state, chunks, half)
-    if step < 1 or not (0 <= b1 < 1 and 0 <= b2 < 1) or eps < 0:
-        raise ValueError(f'step {step}, betas {betas}, eps {eps}: step >= 1, betas in [0, 1) and eps >= 0 needed')
+    if step < 1 or not (0 <= b1 < 1 and 0 <= b2 < 1) or not (eps == 0 or eps >= 1.2e-38):
+        raise ValueError(f'step {step}, betas {betas}, eps {eps}: step >= 1, betas in [0, 1) and eps 0 or a normal f32 number needed')
     if not 0 <= noise < 1 << 32:
         raise ValueError('noise is a 32-bit key')
     d, n, ns, nc = param.get_device(), param.numel(), m8.numel(), start.numel()

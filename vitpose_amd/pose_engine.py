@@ -152,7 +152,7 @@ class PoseEngine:
         if B < 1:
             raise ValueError('empty batch')
         if fp8 is None:
-            fp8 = self.fp8 and not exact
+            fp8 = self.fp8 and not exact and not fold_ln
         elif fp8 and (exact or fold_ln):
             raise ValueError('fp8 excludes exact and fold_ln: one evaluation path at a time')
         fold = (self.fold_layernorm if fold_ln is None else fold_ln) and not exact and not fp8 and self.vit.ln_fold_supported()
