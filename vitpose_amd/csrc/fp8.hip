@@ -10,6 +10,7 @@
 // full f32).  That is 5e-5 of the result's norm on data with a wide spread, against 2e-3 for the bf16 rounding of the result
 // and 3e-2 for the rounding of the operands to e4m3.
 #include <algorithm>
+#include <cmath>
 
 #include "common.h"
 #include "vitpose_hip.h"
@@ -659,49 +660,49 @@ int launch_narrow(int shape, const vp_fp8_args* g, const T* x, long ldx, int K, 
     return launch_narrow<T, 2, 4>(g, x, ldx, K, stream);
 }
 
-// Which kernel: the few-rows kernels by how many operand bytes a K step costs a CU (tile rows + columns; rows that have to be
-// rounded on the way count 2.7 times, in f32 four times), a round of 256 workgroups at a time, the 128 x 128 tile the same
-// way at 0.8 of that.  Where the chip is full of them the tiles' own ratio counts: a round of 256 x 256 tiles takes 2.75 times one
-// of 128 x 128 and does four times the work (24576 x 1280 x 5120: 160 us against 201; 12288 x 4096 x 1024: 61 / 79; at 3000 x
-// 2000 x 3000, a third of a round: 32 / 34).  Measured, us at 16 / 192 / 768 / 1536 rows of K 5120, N 1280, rows given as codes:
-// 16 x 16 6.6 / 20 / 69 / 136, 16 x 32 8.9 / 16 / 55 / 102, 32 x 32 9.8 / 12 / 38 / 73, 32 x 64 15 / 17 / 30 / 57, 128 x 128 29 /
-// 32 / 33 / 34, 256 x 256 59 / 61 / 63 / 63; K 1000, N 777: 3.3 / 5.2 / 12 / 20, 3.8 / 5.2 / 9.4 / 16, 4.0 / 4.5 / 8.4 / 14, 5.1 / 5.7 /
-// 8.6 / 12, 7.9 / 12 / 12 / 13.
+// Which kernel: the one that a simple model of the time, in us, puts first.
+//   Few rows: 31 ns per 1000 of K and operand row that a workgroup reads (tile rows + columns; rows that have to be rounded on
+//   the way count 2.7 times, in f32 four times), a round of 256 workgroups at a time.  Measured, us at 16 / 192 / 768 / 1536 rows of
+//   K 5120, N 1280, rows given as codes: 16 x 16 6.6 / 20 / 69 / 136, 16 x 32 8.9 / 16 / 55 / 102, 32 x 32 9.8 / 12 / 38 / 73, 32 x 64
+//   15 / 17 / 30 / 57, 128 x 128 29 / 32 / 33 / 34, 256 x 256 59 / 61 / 63 / 63; K 1000, N 777: 3.3 / 5.2 / 12 / 20, 3.8 / 5.2 / 9.4 /
+//   16, 4.0 / 4.5 / 8.4 / 14, 5.1 / 5.7 / 8.6 / 12, 7.9 / 12 / 12 / 13.
+//   Tiles: a round of 256 takes a part for its beginning and its stores, more with a GELU, and a part per K tile; of the
+//   128 x 128 tiles two share a CU, so a last round that is not full costs half of what it lacks.  Measured, us, 128 x 128 / 256 x 256: 24576 x 1280 x 5120 201 /
+//   160, 24576 x 3840 x 1280 178 / 149, 12288 x 2304 x 768 38 / 37, 6144 x 1024 x 4096 42 / 64; with a GELU 24576 x 5120 x 1280 273 /
+//   241, 6144 x 4096 x 1024 50 / 54.
 enum { TILE_128 = 4, TILE_256 = 5 };
 constexpr int kRows[4] = {16, 16, 32, 32}, kCols[4] = {16, 32, 32, 64};
 
-double narrow_cost(int shape, int M, int N, double row_weight) {
-    const long wgs = (long)cdiv(M, kRows[shape]) * cdiv(N, kCols[shape]);
-    return (double)((wgs + 255) / 256) * (kRows[shape] * row_weight + kCols[shape]);
-}
-
-int best_narrow(int M, int N, double row_weight, double& cost) {
+int best_narrow(int M, int N, int K, double row_weight, double further, double& us) {
     int best = 0;
-    cost = narrow_cost(0, M, N, row_weight);
-    for (int s = 1; s < 4; ++s) {
-        const double c = narrow_cost(s, M, N, row_weight);
-        if (c < cost) { cost = c; best = s; }
+    for (int s = 0; s < 4; ++s) {
+        const long wgs = (long)cdiv(M, kRows[s]) * cdiv(N, kCols[s]);
+        const double rounds = (double)((wgs + 255) / 256);
+        const double t = rounds * (kRows[s] * row_weight + kCols[s]) * K * 31e-6 + (rounds - 1) * further;
+        if (s == 0 || t < us) { us = t; best = s; }
     }
     return best;
 }
 
-int product_kernel(int M, int N, double& cost) {
-    const int s = best_narrow(M, N, 1.0, cost);
-    const double w128 = std::max(1.0, (double)cdiv(M, 128) * cdiv(N, 128) / 256);
+int product_kernel(int M, int N, int K, int act, double& us) {
+    const int s = best_narrow(M, N, K, 1.0, 0.0, us), kb = cdiv(K, BLK);
+    const double tiles = (double)cdiv(M, 128) * cdiv(N, 128) / 256, w128 = std::max(1.25, (tiles + 2 * std::ceil(tiles / 2)) / 2);
     const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
-    const double tile = 205 * std::min(w128, 2.75 * w256);
-    if (cost <= tile) return s;
-    cost = tile;
-    return w128 <= 2.75 * w256 ? TILE_128 : TILE_256;
+    const double t128 = w128 * (1.7 + 0.63 * kb + 1.2 * act), t256 = w256 * (7.0 + 1.84 * kb + 5.0 * act);
+    const double tile = std::min(t128, t256);
+    if (us <= tile) return s;
+    us = tile;
+    return t128 <= t256 ? TILE_128 : TILE_256;
 }
 
-// The few-rows kernel that rounds its rows itself, or -1: a launch of the quantizer costs about 4 us more, a unit of the costs above
-// 31 ns per 1000 of K.
+// The few-rows kernel that rounds its rows itself, or -1: a launch of the quantizer costs about 4 us more, a further round of
+// workgroups that begin by rounding 2 us (us, one launch / two: 192 x 4096 x 1024 14.8 / 11.5, 384 x 2304 x 768 13.0 / 10.8,
+// 384 x 777 x 1000 7.5 / 8.5, 1 x 5120 x 1280 5.1 / 5.6).
 int fused_kernel(int M, int N, int K, int dtype) {
     double fused, split;
-    const int s = best_narrow(M, N, dtype == VP_F32 ? 4.0 : 2.7, fused);
-    product_kernel(M, N, split);
-    return fused * K <= split * K + 4.0 / 31e-6 ? s : -1;
+    const int s = best_narrow(M, N, K, dtype == VP_F32 ? 4.0 : 2.7, 2.0, fused);
+    product_kernel(M, N, K, 0, split);
+    return fused <= split + 4.0 ? s : -1;
 }
 
 template <int BM, int BN, int WN, int RING>
@@ -726,8 +727,8 @@ extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
     // Codes: 128 x 128 tiles, two of which share a CU: one's largest magnitudes, rounding and GELU, 20 us of a 256 x 256 tile, pass
     // under the other's matrix instructions (6144 x 4096 x 1024: 52 us
     // against 65; 24576 x 5120 x 1280: 277 against 301).
-    double cost;
-    const int which = g->out_dtype == VP_E4M3 ? TILE_128 : product_kernel(g->M, g->N, cost);
+    double us;
+    const int which = g->out_dtype == VP_E4M3 ? TILE_128 : product_kernel(g->M, g->N, g->K, g->act, us);
     if (which < TILE_128) return launch_narrow<uint8_t>(which, g, (const uint8_t*)g->xq, g->ldx, g->K, stream);
     if (which == TILE_256) return launch_tile<256, 256, 4, 18>(g, stream);
     // one workgroup a CU: eight waves; two: four waves each (3000 x 2000 x 3000: 31 us against 34; 192 x 4096 x 1024: 8.5 / 8.1)
