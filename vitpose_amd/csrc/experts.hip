@@ -162,19 +162,19 @@ __device__ __forceinline__ void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N_) : "memory");
 }
 
-constexpr int LIST = 2048;   // entries of the row list that a dW workgroup keeps in LDS at a time
 
 // BM x BN tile by eight waves: waves 0-3 (2 x 2 blocks of BM / 2 x BN / 2) take the first 32 reduction steps of every K tile,
 // waves 4-7 the other 32, so a CU has two waves per SIMD on blocks as large as four would have; the halves meet through LDS
 // once at the end.  S stages: while K tile t is multiplied, the loads of t + 1 .. t + S - 1 are in flight (what bounds
 // these products is the time a load takes, not the rate: with two stages the 128 x 128 tile needed 1 us per K tile for 0.2 us of
 // matrix instructions).  One barrier per K tile.  Loads past the end fetch zeros, so that the counted waits hold.
-template <int WHAT, int BM, int BN, int S>
-__global__ __launch_bounds__(THREADS, 2) void grouped_kernel(Args a, int tiles_j, int tiles_i) {
+template <int WHAT, int BM, int BN, int S, int PER_CU = 1>
+__global__ __launch_bounds__(THREADS, 2 * PER_CU) void grouped_kernel(Args a, int tiles_j, int tiles_i) {
     constexpr bool XK = WHAT == DW, YK = WHAT != FWD;
     constexpr int UX = BM / 64, UY = BN / 64, U = UX + UY, FM = BM / 32, FN = BN / 32, FH = FM / 2, STAGE = U * UNIT;
     constexpr int SWAP = 8 * FH * FN * 1024, PITCH = BN + 16, PATCH = 16 * FH * PITCH;
     constexpr int BYTES = S * STAGE > SWAP ? S * STAGE : SWAP;
+    constexpr int LIST = 2048 / PER_CU;                    // entries of the row list that a dW workgroup keeps in LDS at a time
     static_assert(8 * PATCH <= BYTES, "the result patches reuse the stages");
     __shared__ __attribute__((aligned(16))) char lds[BYTES];
     __shared__ int list[XK ? LIST : 1];
@@ -767,13 +767,16 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_kernel(const int* __
 
 // The same for up to FEW_E experts: a lane owns a run of consecutive rows and a counter per key (in LDS, its own column: no
 // conflicts), so that a row costs a lane a few instructions instead of costing a wave a round of votes.  12288 rows, six
-// experts: 7.4 us against 13 us for the votes.
-constexpr int FEW_E = 15;
+// experts: 6.1 us (7.4 with the list written row by row) against 13 us for the votes.
+// The list itself is put together in LDS where it fits, so that what leaves are whole lines.
+constexpr int FEW_E = 15, FEW_ROWS = 16384;
 
 __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int* __restrict__ expert, int T, int E,
                                                                        int* __restrict__ rows, int* __restrict__ offsets) {
     __shared__ int count[FEW_E + 1][SORT_THREADS];
     __shared__ int total[SORT_WAVES][FEW_E + 1];
+    __shared__ int list[FEW_ROWS];
+    const bool staged = T <= FEW_ROWS;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = E + 1;
     const int each = ((T + SORT_THREADS - 1) / SORT_THREADS + 3) & ~3;      // whole sixteen-byte loads
     const int t0 = min((long)tid * each, (long)T), t1 = min(t0 + each, T);
@@ -836,9 +839,14 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int
         for (int d = 0; d < SORT_DEEP; ++d)
             if (t + d < t1) {
                 const int at = __hip_atomic_fetch_add(&count[key[d]][tid], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                rows[total[wave][key[d]] + at] = t + d;
+                const int to = total[wave][key[d]] + at;
+                if (staged) list[to] = t + d;
+                else rows[to] = t + d;
             }
     }
+    if (!staged) return;
+    __syncthreads();
+    for (int i = tid; i < T; i += SORT_THREADS) rows[i] = list[i];
 }
 
 constexpr int MAX_T = 1 << 30;                         // row numbers, and a tile or a run behind them, stay in 32 bits
@@ -917,29 +925,26 @@ int launch_dx(const vp_grouped_args* g, hipStream_t stream) {
     VP_LAUNCH_RET();
 }
 
-template <int WHAT, int BM, int S>
+template <int WHAT, int BM, int S, int PER_CU = 1>
 int launch_rows(const vp_grouped_args* g, hipStream_t stream) {
     constexpr int BN = 128;
     const int tj = cdiv(WHAT == FWD ? g->N : g->K, BN);
     const long grid = (long)row_tiles(g, BM) * tj;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
-    hipLaunchKernelGGL((grouped_kernel<WHAT, BM, BN, S>), dim3((unsigned)grid), dim3(THREADS), 0, stream, make_args(g), tj, 0);
+    hipLaunchKernelGGL((grouped_kernel<WHAT, BM, BN, S, PER_CU>), dim3((unsigned)grid), dim3(THREADS), 0, stream, make_args(g), tj, 0);
     VP_LAUNCH_RET();
 }
 
-template <int BM, int BN, int S>
-void launch_dw(const Args& a, hipStream_t stream, long grid, int tj, int ti) {
-    hipLaunchKernelGGL((grouped_kernel<DW, BM, BN, S>), dim3((unsigned)grid), dim3(THREADS), 0, stream, a, tj, ti);
-}
-
-// dW tiles of 64 rows of N waste less where N ends in the first half of a 128-row tile; a tile costs a tenth more there
-// (us at 6144 rows of 320 x 5120 / 12288 of 256 x 4096, six experts: 64 x 256 tiles 41 / 74, 128 x 128 47 / 62)
-bool dw_short(int N) { return cdiv(N, 64) * 11 < cdiv(N, 128) * 20; }
+// dW in tiles of 64 x 128, two of which share a CU: one's loads and stores pass under the other's sums, and an extent of N that
+// ends in the first half of 128 wastes nothing.  us at 32 / 768 / 5003 / 12288 rows against one 128 x 128 (N 320: 64 x 256) tile a CU:
+// 5120 x 320, six experts 19 / 21 / 40 / 91 against 22 / 25 / 40 / 93; 4096 x 256 13 / 16 / 28 / 63, 15 / 17 / 29 / 64; 1024 x 1024, 24
+// experts 33 / 42 / 54 / 76, 35 / 45 / 60 / 76; 512 x 512, 48 experts 22 / 28 / 32 / 37, 22 / 28 / 35 / 39.
+constexpr int DW_BM = 64, DW_BN = 128;
 
 // The rows are cut into slices where the tiles alone would leave CUs without work; a slice has at least 512 rows.
 int dw_slices(int T, int E, int N, int K) {
-    const long tiles = dw_short(N) ? (long)E * cdiv(N, 64) * cdiv(K, 256) : (long)E * cdiv(N, 128) * cdiv(K, 128);
-    const long s = std::min<long>(256 / std::max<long>(tiles, 1), (T + 511) / 512);
+    const long tiles = (long)E * cdiv(N, DW_BM) * cdiv(K, DW_BN);
+    const long s = std::min<long>(512 / std::max<long>(tiles, 1), (T + 511) / 512);
     return s < 1 ? 1 : (int)s;
 }
 
@@ -953,21 +958,25 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     VP_CHECK_ARG(g->stride_w % 8 == 0 && (!g->bias || (aligned16(g->bias) && g->stride_b % 4 == 0)));
     // The kernels differ in how many bytes a CU has to fetch: a workgroup reads tile rows + tile columns operand rows, 256 run
     // at a time, and a CU takes in some 50 KB a microsecond, whoever else is running -- twice that where the loads go to LDS
-    // four K tiles ahead, as in the 128 x 128 kernel.  The smallest (rounds x operand rows) wins; it ranks what was measured
+    // several K tiles ahead, as in the 128-wide tiles.  The smallest (rounds x operand rows) wins; it ranks what was measured
     // right.  K 4096, N 256, 6 experts, us at 1 / 192 / 768 / 1536 rows: 16 x 16 7.1 / 17.9 / 31.5 / 52, 16 x 32 10.9 / 15.0 / 25 / 46,
-    // 32 x 32 12.2 / 18.6 / 18.9 / 34, 32 x 64 19.0 / 25.4 / 25.4 / 25.8, 128 x 128 31.1 / 32.0 / 32.4 / 32.5.  K 1024, N 1024, 24 experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 /
-    // 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
-    const auto cost = [&](int tm, int tn, int weight) {
-        const long tiles = g->T / tm + (std::min(g->E, g->T) + 1) / 2;         // experts' last tiles: half full on average
-        return (tiles * cdiv(g->N, tn) + 255) / 256 * (tm + tn) * weight;
+    // 32 x 32 12.2 / 18.6 / 18.9 / 34, 32 x 64 19.0 / 25.4 / 25.4 / 25.8, 128 x 128 31.1 / 32.0 / 32.4 / 32.5.  K 1024, N 1024, 24
+    // experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 / 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
+    // Of the 64 x 128 tiles two share a CU: 192 rows a CU's worth up to 256 of them, half as much again where the CUs fill up
+    // once, 250 a full round of 512 of many.  64 x 128 / 128 x 128, us, K 4096, N 256 at 2500 / 6144 / 12288 rows: 24 / 33, 25 / 34, 41 /
+    // 37; K 5120, N 320 at 5003 / 6144: 31 / 41, 49 / 41; K 2048, N 1024, 8 experts at 5003 / 12288: 35 / 40, 77 / 84.
+    const auto tiles = [&](int tm, int tn) {
+        return (g->T / tm + (std::min(g->E, g->T) + 1) / 2) * (long)cdiv(g->N, tn);     // experts' last tiles: half full on average
     };
-    const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), tile = cost(128, 128, 1);
-    const long best = std::min({c11, c12, c22, c24, tile});
+    const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
+    const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), large = cost(128, 128, 1);
+    const long n64 = tiles(64, 128), last = n64 % 512, c64 = n64 / 512 * 250 + (last == 0 ? 0 : last <= 256 ? 192 : 280);
+    const long best = std::min({c11, c12, c22, c24, large, c64});
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
     if (best == c22) return launch_narrow<2, 2>(g, stream);
     if (best == c24) return launch_narrow<2, 4>(g, stream);
-    return launch_rows<FWD, 128, 4>(g, stream);
+    return best == c64 ? launch_rows<FWD, 64, 3, 2>(g, stream) : launch_rows<FWD, 128, 4>(g, stream);
 }
 
 extern "C" int vp_grouped_dgrad(const vp_grouped_args* g, hipStream_t stream) {
@@ -994,8 +1003,7 @@ extern "C" int vp_grouped_wgrad(const vp_grouped_args* g, float* dw, float* db, 
     VP_CHECK_ARG(dw && aligned16(dw) && (g->T == 0 || (g->dy && g->x && aligned16(g->dy) && aligned16(g->x))));
     VP_CHECK_ARG(g->ldx >= g->K && g->ldy >= g->N && g->ldx % 8 == 0 && g->ldy % 8 == 0 && (!db || aligned16(db)));
     Args a = make_args(g);
-    const bool narrow = dw_short(g->N);
-    const int ti = cdiv(g->N, narrow ? 64 : 128), tj = cdiv(g->K, narrow ? 256 : 128);
+    const int ti = cdiv(g->N, DW_BM), tj = cdiv(g->K, DW_BN);
     a.slices = dw_slices(g->T, g->E, g->N, g->K);
     const size_t need = a.slices == 1 ? 0 : (size_t)a.slices * g->E * g->N * ((size_t)g->K + (db ? 1 : 0)) * 4;
     VP_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && aligned16(workspace)));
@@ -1004,8 +1012,7 @@ extern "C" int vp_grouped_wgrad(const vp_grouped_args* g, float* dw, float* db, 
     a.db = a.slices == 1 ? db : (db ? (float*)workspace + a.slices * n : nullptr);
     const long grid = ((long)g->E * tj * a.slices + 7) / 8 * 8 * ti;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
-    if (narrow) launch_dw<64, 256, 3>(a, stream, grid, tj, ti);
-    else launch_dw<128, 128, 4>(a, stream, grid, tj, ti);
+    hipLaunchKernelGGL((grouped_kernel<DW, DW_BM, DW_BN, 3, 2>), dim3((unsigned)grid), dim3(THREADS), 0, stream, a, tj, ti);
     if (a.slices > 1) {
         const int blocks = (int)(n / 4 < 2048L * 256 ? cdiv(n / 4, 256) : 2048);
         hipLaunchKernelGGL(slice_sum_kernel, dim3(blocks), dim3(256), 0, stream, a.dw, dw, n / 4, a.slices);
