@@ -962,7 +962,7 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // right.  K 4096, N 256, 6 experts, us at 1 / 192 / 768 / 1536 rows: 16 x 16 7.1 / 17.9 / 31.5 / 52, 16 x 32 10.9 / 15.0 / 25 / 46,
     // 32 x 32 12.2 / 18.6 / 18.9 / 34, 32 x 64 19.0 / 25.4 / 25.4 / 25.8, 128 x 128 31.1 / 32.0 / 32.4 / 32.5.  K 1024, N 1024, 24
     // experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 / 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
-    // Of the 64 x 128 tiles two share a CU: 192 rows a CU's worth up to 256 of them, half as much again where the CUs fill up
+    // Of the 64 x 128 tiles two share a CU: 180 rows up to 256 of them, half as much again where the CUs fill up
     // once, 250 a full round of 512 of many.  64 x 128 / 128 x 128, us, K 4096, N 256 at 2500 / 6144 / 12288 rows: 24 / 33, 25 / 34, 41 /
     // 37; K 5120, N 320 at 5003 / 6144: 31 / 41, 49 / 41; K 2048, N 1024, 8 experts at 5003 / 12288: 35 / 40, 77 / 84.
     const auto tiles = [&](int tm, int tn) {
@@ -970,7 +970,7 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     };
     const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
     const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), large = cost(128, 128, 1);
-    const long n64 = tiles(64, 128), last = n64 % 512, c64 = n64 / 512 * 250 + (last == 0 ? 0 : last <= 256 ? 192 : 280);
+    const long n64 = tiles(64, 128), last = n64 % 512, c64 = n64 / 512 * 250 + (last == 0 ? 0 : last <= 256 ? 180 : 280);
     const long best = std::min({c11, c12, c22, c24, large, c64});
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
