@@ -666,10 +666,10 @@ int launch_narrow(int shape, const vp_fp8_args* g, const T* x, long ldx, int K, 
 //   K 5120, N 1280, rows given as codes: 16 x 16 6.6 / 20 / 69 / 136, 16 x 32 8.9 / 16 / 55 / 102, 32 x 32 9.8 / 12 / 38 / 73, 32 x 64
 //   15 / 17 / 30 / 57, 128 x 128 29 / 32 / 33 / 34, 256 x 256 59 / 61 / 63 / 63; K 1000, N 777: 3.3 / 5.2 / 12 / 20, 3.8 / 5.2 / 9.4 /
 //   16, 4.0 / 4.5 / 8.4 / 14, 5.1 / 5.7 / 8.6 / 12, 7.9 / 12 / 12 / 13.
-//   Tiles: a round of 256 takes a part for its beginning and its stores, more with a GELU, and a part per K tile; of the
+//   Tiles: a round of 256 takes a part for its beginning and its stores, more with a GELU or a residual, and a part per K tile; of the
 //   128 x 128 tiles two share a CU, so a last round that is not full costs half of what it lacks.  Measured, us, 128 x 128 / 256 x 256: 24576 x 1280 x 5120 201 /
 //   160, 24576 x 3840 x 1280 178 / 149, 12288 x 2304 x 768 38 / 37, 6144 x 1024 x 4096 42 / 64; with a GELU 24576 x 5120 x 1280 273 /
-//   241, 6144 x 4096 x 1024 50 / 54.
+//   241, 6144 x 4096 x 1024 50 / 54; with a residual 24576 x 1280 x 5120 229 / 201, 12288 x 768 x 768 29 / 31.
 enum { TILE_128 = 4, TILE_256 = 5 };
 constexpr int kRows[4] = {16, 16, 32, 32}, kCols[4] = {16, 32, 32, 64};
 
@@ -684,14 +684,18 @@ int best_narrow(int M, int N, int K, double row_weight, double further, double& 
     return best;
 }
 
-int product_kernel(int M, int N, int K, int act, double& us) {
+int product_kernel(int M, int N, int K, int act, bool resid, double& us) {
     const int s = best_narrow(M, N, K, 1.0, 0.0, us), kb = cdiv(K, BLK);
     const double tiles = (double)cdiv(M, 128) * cdiv(N, 128) / 256, w128 = std::max(1.25, (tiles + 2 * std::ceil(tiles / 2)) / 2);
     const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
-    const double t128 = w128 * (1.7 + 0.63 * kb + 1.2 * act), t256 = w256 * (7.0 + 1.84 * kb + 5.0 * act);
+    double t128 = w128 * (1.7 + 0.63 * kb + 1.2 * act), t256 = w256 * (7.0 + 1.84 * kb + 5.0 * act);
     const double tile = std::min(t128, t256);
     if (us <= tile) return s;
     us = tile;
+    if (resid) {                        // (the two tiles add up in one order: a residual does not change the product's bits)
+        t128 += 1.5 * w128;
+        t256 += 10.0 * w256;
+    }
     return t128 <= t256 ? TILE_128 : TILE_256;
 }
 
@@ -701,7 +705,7 @@ int product_kernel(int M, int N, int K, int act, double& us) {
 int fused_kernel(int M, int N, int K, int dtype) {
     double fused, split;
     const int s = best_narrow(M, N, K, dtype == VP_F32 ? 4.0 : 2.7, 2.0, fused);
-    product_kernel(M, N, K, 0, split);
+    product_kernel(M, N, K, 0, false, split);
     return fused <= split + 4.0 ? s : -1;
 }
 
@@ -728,7 +732,7 @@ extern "C" int vp_gemm_fp8(const vp_fp8_args* g, hipStream_t stream) {
     // under the other's matrix instructions (6144 x 4096 x 1024: 52 us
     // against 65; 24576 x 5120 x 1280: 277 against 301).
     double us;
-    const int which = g->out_dtype == VP_E4M3 ? TILE_128 : product_kernel(g->M, g->N, g->K, g->act, us);
+    const int which = g->out_dtype == VP_E4M3 ? TILE_128 : product_kernel(g->M, g->N, g->K, g->act, g->resid != nullptr, us);
     if (which < TILE_128) return launch_narrow<uint8_t>(which, g, (const uint8_t*)g->xq, g->ldx, g->K, stream);
     if (which == TILE_256) return launch_tile<256, 256, 4, 18>(g, stream);
     // one workgroup a CU: eight waves; two: four waves each (3000 x 2000 x 3000: 31 us against 34; 192 x 4096 x 1024: 8.5 / 8.1)
