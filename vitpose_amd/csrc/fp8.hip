@@ -55,7 +55,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
     }
 }
 
-// ---- rows: sixteen lanes hold a block of one row ----
+// ---- rows: sixteen lanes hold a block of one row; HBM-bound: 24576 x 5120 from bf16 75 us = 5.0 TB/s ----
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, long ldx, int M, int K, int KB,
                                                             uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -82,6 +82,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict_
 }
 
 // ---- rows behind a LayerNorm: a wave holds a row, four blocks of it at a time, and the LayerNorm's weights ----
+// Statistics in f32, the variance from differences.  HBM-bound: the next row is on its way while one is rounded; 24576 x 1280 30 us =
+// 5.3 TB/s (the LayerNorm to bf16 and the rounding as two launches: 31 + 19).
 template <int NB>
 __global__ __launch_bounds__(256) void layernorm_rows_kernel(const float* __restrict__ x, const float* __restrict__ gamma,
                                                              const float* __restrict__ beta, float eps, int M, int E, int KB,
@@ -270,7 +272,8 @@ __device__ __forceinline__ f32x4 load_bias(const Args& a, int j) {
 // 16.8.  LDS is a ring of RING units: behind the K tile being multiplied and the next one, the loads of RING - 2 U more units
 // are in flight (with none, the 256 x 256 tile waits for every burst of loads: 2 us a K tile for 0.9 of matrix instructions).
 // A lane's accumulators are in f32 units; a K tile's product starts from zero and is added with its block's scale (one FMA
-// a value: half of the matrix instructions' time, on another unit).
+// a value: half of the matrix instructions' time, on another unit).  Measured: 24576 x 1280 x 5120 160 us = 2.0 PFLOP/s on 256 x 256
+// tiles, 201 on 128 x 128.
 // OUT: what is stored (the dtype tag): one kernel each, or the registers of one epilogue are spilled in another.
 template <int BM, int BN, int WN, int RING, int OUT>
 __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
@@ -481,7 +484,8 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
 // A workgroup computes 16 FM rows x 16 FN columns; its eight waves take every eighth block of K straight from memory into
 // matrix-instruction operands, and the eight partial tiles are added up in LDS in a fixed order.  Rows in f32 or bf16 are
 // rounded to e4m3 on the way (a block of a row lies in four lanes): the same codes and scales as the quantizer's, without
-// its launch; every workgroup of a row does it again, which few rows can afford.
+// its launch; every workgroup of a row does it again, which few rows can afford.  Measured: one row, 1280 -> 5120 5.5 us; 192 rows of
+// codes, 1024 -> 4096 with a GELU 9.6.
 template <typename T, int FM, int FN>
 __global__ __launch_bounds__(512, 2) void fp8_narrow_kernel(Args a, const T* __restrict__ x, long ldx, int K, int tiles_n) {
     constexpr int TM = 16 * FM, TN = 16 * FN;
