@@ -365,3 +365,36 @@ def test_layernorm_refusals():
             fp8.layernorm_rows(*bad)
     with pytest.raises(RuntimeError):
         fp8.layernorm_rows(x, w.cpu(), w)
+
+
+def test_codes_from_layernorm_to_product_on_another_stream_and_in_replayed_graphs():
+    g = torch.Generator().manual_seed(4)
+    M, E, N = 300, 264, 520
+    xs = [torch.randn(M, E, generator=g).cuda() * k for k in (1.0, 3.0, 0.2)]
+    gamma, beta = torch.randn(E, generator=g).cuda(), torch.randn(E, generator=g).cuda()
+    w1, w2 = fp8.quantize_weight(torch.randn(N, E, generator=g).cuda()), fp8.quantize_weight(torch.randn(E, N, generator=g).cuda())
+
+    def run(x):
+        h = fp8.product(*fp8.layernorm_rows(x, gamma, beta), *w1, act='gelu', out_dtype=torch.float8_e4m3fn)
+        return fp8.product(*h, *w2, out_dtype=torch.float32, resid=x)
+    want = [run(x) for x in xs]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    static = xs[0].clone()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        got = run(static)
+    side.synchronize()
+    assert torch.equal(got, want[0])
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(static)
+        graphs.append((graph, out))
+    for k in (1, 2, 0, 1):
+        static.copy_(xs[k])
+        for graph, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want[k]) for _, out in graphs) and torch.equal(run(xs[k]), want[k])

@@ -211,7 +211,8 @@ class _GroupedLinear(torch.autograd.Function):
 class ExpertLinear(nn.Module):
     """num_expert Linears of one shape, one per row: y[t] = x[t] @ weight[expert[t]].T + bias[expert[t]], zeros where
     expert[t] is not in [0, num_expert).  f32 master parameters (torch optimizers apply); every call rounds them to bf16
-    once.  x bf16 [T, in_features], expert int32 [T]."""
+    once.  x bf16 [T, in_features], expert int32 [T].  A backward pass may be captured into a graph while no graph of an eager
+    pass over the same parameters is alive (torch ends the process otherwise)."""
 
     def __init__(self, num_expert, in_features, out_features, bias=True, device=None):
         super().__init__()

@@ -106,7 +106,8 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
     run of at most 2048 consecutive elements of one tensor (starts and lengths multiples of 4, state starts multiples
     of 128, no overlaps; an entry that leaves the buffers is skipped);  step: number of this step, from 1;  noise: key
     of this step's random numbers (`noise_key`).  max_grad_norm > 0 clips the gradients of the table's elements by their
-    norm first.  Everything is updated in place on the current stream; nothing synchronises."""
+    norm first.  Everything is updated in place on the current stream; nothing synchronises.  lr, step and noise are arguments
+    of the launch: a captured graph repeats the ones that it was captured with."""
     m8, ms, r8, rs = state
     start, length, lr_scale, decay, state_start = chunks or (None,) * 5
     b1, b2 = betas
