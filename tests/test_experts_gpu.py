@@ -345,3 +345,23 @@ def test_a_gradient_off_its_sixteen_bytes_and_a_layer_without_bias():
             want[k] += dy[t].cpu().double()[:, None] * x[t].cpu().double()
     # two products of bf16 numbers at most are added in f32
     assert (layer.weight.grad.cpu().double() - want).abs().max() <= 4 * 2.0 ** -24 * 16
+
+
+@pytest.mark.parametrize('T,E,K,N,listed', [(5003, 8, 72, 1024, True), (12300, 6, 40, 320, False), (16384, 3, 136, 256, True), (9001, 1, 64, 520, True)])
+def test_forward_products_of_many_rows(T, E, K, N, listed):
+    """Row counts at which the 64-, 128- and 192-row tiles take turns."""
+    g = torch.Generator().manual_seed(T)
+    x, w, b = torch.randn(T, K, generator=g).bfloat16(), torch.randn(E, N, K, generator=g).bfloat16(), torch.randn(E, N, generator=g)
+    ids = torch.randint(-1, E, (T,), generator=g).int()
+    ids[torch.rand(T, generator=g) < 0.4] = 0
+    if not listed:
+        ids = ids.clamp(min=0).sort()[0].int()
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    got = experts.grouped_linear(x.cuda(), w.cuda(), b.cuda(), offsets, rows if listed else None).cpu().double()
+    want, mag = torch.zeros(T, N, dtype=torch.float64), torch.zeros(T, N, dtype=torch.float64)
+    for e in range(E):
+        s = ids == e
+        want[s] = x[s].double() @ w[e].double().t() + b[e].double()
+        mag[s] = x[s].double().abs() @ w[e].double().abs().t() + b[e].double().abs()
+    tol = (K + 4) * 2.0 ** -24 * mag
+    assert ((got - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()

@@ -969,19 +969,23 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 / 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
     // Of the 64 x 128 tiles two share a CU: 180 rows up to 256 of them, half as much again where the CUs fill up
     // once, 250 a full round of 512 of many.  64 x 128 / 128 x 128, us, K 4096, N 256 at 2500 / 6144 / 12288 rows: 24 / 33, 25 / 34, 41 /
-    // 37; K 5120, N 320 at 5003 / 6144: 31 / 41, 49 / 41; K 2048, N 1024, 8 experts at 5003 / 12288: 35 / 40, 77 / 84.
+    // 37; K 5120, N 320 at 5003 / 6144: 31 / 41, 49 / 41; K 2048, N 1024, 8 experts at 5003 / 12288: 35 / 40, 77 / 84.  192 x 128 (three
+    // stages) where it saves rounds, against the best of the others, inputs in memory: K 5120, N 320 at 12288 / 16384 rows 67 / 96,
+    // 119 / 100; K 4096, N 256 at 12288 / 16384 55 / 46, 61 / 79; K 2048, N 1024, 8 experts at 5003 / 16384 32 / 44, 90 / 113.
     const auto tiles = [&](int tm, int tn) {
         return (g->T / tm + (std::min(g->E, g->T) + 1) / 2) * (long)cdiv(g->N, tn);     // experts' last tiles: half full on average
     };
     const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
-    const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), large = cost(128, 128, 1);
+    const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), c128 = cost(128, 128, 1);
+    const long c192 = cost(192, 128, 1);
     const long n64 = tiles(64, 128), last = n64 % 512, c64 = n64 / 512 * 250 + (last == 0 ? 0 : last <= 256 ? 180 : 280);
-    const long best = std::min({c11, c12, c22, c24, large, c64});
+    const long best = std::min({c11, c12, c22, c24, c64, c128, c192});
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
     if (best == c22) return launch_narrow<2, 2>(g, stream);
     if (best == c24) return launch_narrow<2, 4>(g, stream);
-    return best == c64 ? launch_rows<FWD, 64, 3, 2>(g, stream) : launch_rows<FWD, 128, 4>(g, stream);
+    if (best == c64) return launch_rows<FWD, 64, 3, 2>(g, stream);
+    return best == c128 ? launch_rows<FWD, 128, 4>(g, stream) : launch_rows<FWD, 192, 3>(g, stream);
 }
 
 extern "C" int vp_grouped_dgrad(const vp_grouped_args* g, hipStream_t stream) {
