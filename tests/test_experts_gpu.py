@@ -365,3 +365,18 @@ def test_forward_products_of_many_rows(T, E, K, N, listed):
         mag[s] = x[s].double().abs() @ w[e].double().abs().t() + b[e].double().abs()
     tol = (K + 4) * 2.0 ** -24 * mag
     assert ((got - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()
+
+
+@pytest.mark.parametrize('T', [1, 63, 1910, 1911, 2021, 5210, 5211, 16383, 16384, 16385, 40001])
+@pytest.mark.parametrize('E', [1, 2, 15, 16, 31, 32, 300])
+def test_rows_are_ordered_whichever_kernel_does_it(T, E):
+    g = torch.Generator().manual_seed(T + E)
+    ids = torch.randint(-2, E + 2, (T + 1,), generator=g).int()
+    if E > 2:
+        ids[torch.rand(T + 1, generator=g) < 0.3] = 1
+    for first in (0, 1):                    # on sixteen bytes and off them
+        some = ids[first:first + T]
+        rows, offsets = experts.expert_rows(ids.cuda()[first:first + T], E)
+        key = torch.where((some >= 0) & (some < E), some, torch.full_like(some, E)).long()
+        assert torch.equal(rows.cpu().long(), torch.argsort(key, stable=True))
+        assert torch.equal(offsets.cpu().long(), torch.bincount(key, minlength=E + 1).cumsum(0)[:E + 1] - torch.bincount(key, minlength=E + 1)[:E + 1])

@@ -770,18 +770,22 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_kernel(const int* __
     }
 }
 
-// The same for up to FEW_E experts: a lane owns a run of consecutive rows and a counter per key (in LDS, its own column: no
-// conflicts), so that a row costs a lane a few instructions instead of costing a wave a round of votes.  12288 rows, six
-// experts: 6.1 us (7.4 with the list written row by row) against 13 us for the votes.
-// The list itself is put together in LDS where it fits, so that what leaves are whole lines.
-constexpr int FEW_E = 15, FEW_ROWS = 16384;
+// The same for fewer than FEW_KEYS experts and many rows: a lane owns a run of consecutive rows and a counter per key (in LDS, its
+// own column: no conflicts), so that a row costs a lane a few instructions instead of costing a wave a round of votes; the
+// scans over the lanes, one per key, are what it costs beyond that.  us at 192 / 5003 / 12288 rows, votes against runs: 6 experts 3.4 /
+// 7.1 / 13, 4.9 / 5.5 / 6.2; 24 experts 3.5 / 8.3 / 15.8, 6.9 / 7.9 / 10.0.
+// The list itself is put together in LDS where it fits beside the counters (KEYS of 16, up to 16384 rows), so that what leaves are
+// whole lines.
+constexpr int FEW_KEYS = 32, FEW_ROWS = 16384;
 
+template <int KEYS>
 __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int* __restrict__ expert, int T, int E,
                                                                        int* __restrict__ rows, int* __restrict__ offsets) {
-    __shared__ int count[FEW_E + 1][SORT_THREADS];
-    __shared__ int total[SORT_WAVES][FEW_E + 1];
-    __shared__ int list[FEW_ROWS];
-    const bool staged = T <= FEW_ROWS;
+    constexpr int LIST = KEYS <= 16 ? FEW_ROWS : 1;
+    __shared__ int count[KEYS][SORT_THREADS];
+    __shared__ int total[SORT_WAVES][KEYS];
+    __shared__ int list[LIST];
+    const bool staged = T <= LIST;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = E + 1;
     const int each = ((T + SORT_THREADS - 1) / SORT_THREADS + 3) & ~3;      // whole sixteen-byte loads
     const int t0 = min((long)tid * each, (long)T), t1 = min(t0 + each, T);
@@ -814,6 +818,7 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int
     }
     // (a lane's counters are its own, and LDS works a wave's instructions off in order: no barrier before it reads them
     // back; the additions carry no order between lanes, they are additions because those need no round trip)
+#pragma unroll 4
     for (int k = 0; k < keys; ++k) {
         const int n = count[k][tid], sum = wave_scan(n);
         count[k][tid] = sum - n;
@@ -863,8 +868,9 @@ int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 extern "C" int vp_expert_rows(const int* expert, int T, int E, int* rows, int* offsets, hipStream_t stream) {
     VP_CHECK_ARG(T >= 0 && T <= MAX_T && E >= 1 && offsets && (T == 0 || (expert && rows)));
     if (E > SORT_MAX_E) return VP_ERR_UNSUPPORTED;
-    if (E <= FEW_E) {
-        hipLaunchKernelGGL(expert_rows_few_kernel, dim3(1), dim3(SORT_THREADS), 0, stream, expert, T, E, rows, offsets);
+    if (E < FEW_KEYS && T > 1800 + 110 * E) {       // (where the two measured the same)
+        auto kernel = E < 16 ? expert_rows_few_kernel<16> : expert_rows_few_kernel<FEW_KEYS>;
+        hipLaunchKernelGGL(kernel, dim3(1), dim3(SORT_THREADS), 0, stream, expert, T, E, rows, offsets);
         VP_LAUNCH_RET();
     }
     int bits = 1;
