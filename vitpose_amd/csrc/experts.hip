@@ -170,7 +170,7 @@ __device__ __forceinline__ void wait_vm() {
 // zeros, so that the counted waits hold.  PER_CU workgroups share a CU.
 // What bounds it is what a CU takes in, 51 KB a microsecond from memory and 60 from caches, whatever the depth and however many
 // CUs are at it: without its LDS reads and matrix instructions the loop takes 40 us instead of 41.  Measured, inputs in memory:
-// forward 12288 x 256 x 4096 46 us = 560 TFLOP/s; 6144 rows of 320 x 5120: forward 51, dW 44 us (39 MB written).
+// forward 12288 x 256 x 4096 46 us = 560 TFLOP/s; 6144 rows of 320 x 5120: forward 43, dW 44 us (39 MB written).
 template <int WHAT, int BM, int BN, int S, int PER_CU = 1>
 __global__ __launch_bounds__(THREADS, 2 * PER_CU) void grouped_kernel(Args a, int tiles_j, int tiles_i) {
     constexpr bool XK = WHAT == DW, YK = WHAT != FWD;
@@ -936,9 +936,8 @@ int launch_dx(const vp_grouped_args* g, hipStream_t stream) {
     VP_LAUNCH_RET();
 }
 
-template <int WHAT, int BM, int S, int PER_CU = 1>
+template <int WHAT, int BM, int S, int PER_CU = 1, int BN = 128>
 int launch_rows(const vp_grouped_args* g, hipStream_t stream) {
-    constexpr int BN = 128;
     const int tj = cdiv(WHAT == FWD ? g->N : g->K, BN);
     const long grid = (long)row_tiles(g, BM) * tj;
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
@@ -973,24 +972,25 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // right.  K 4096, N 256, 6 experts, us at 1 / 192 / 768 / 1536 rows: 16 x 16 7.1 / 17.9 / 31.5 / 52, 16 x 32 10.9 / 15.0 / 25 / 46,
     // 32 x 32 12.2 / 18.6 / 18.9 / 34, 32 x 64 19.0 / 25.4 / 25.4 / 25.8, 128 x 128 31.1 / 32.0 / 32.4 / 32.5.  K 1024, N 1024, 24
     // experts at 1 / 96 / 768 rows: 4.3 / 20 / 49, 5.6 / 17.8 / 41, 6.4 / 22.5 / 44, 7.4 / 15.5 / 33, 11.6 / 14.1 / 15.3.
-    // Of the 64 x 128 tiles two share a CU: 180 rows up to 256 of them, half as much again where the CUs fill up
-    // once, 250 a full round of 512 of many.  64 x 128 / 128 x 128, us, K 4096, N 256 at 2500 / 6144 / 12288 rows: 24 / 33, 25 / 34, 41 /
-    // 37; K 5120, N 320 at 5003 / 6144: 31 / 41, 49 / 41; K 2048, N 1024, 8 experts at 5003 / 12288: 35 / 40, 77 / 84.  192 x 128 (three
-    // stages) where it saves rounds, against the best of the others, inputs in memory: K 5120, N 320 at 12288 / 16384 rows 67 / 96,
-    // 119 / 100; K 4096, N 256 at 12288 / 16384 55 / 46, 61 / 79; K 2048, N 1024, 8 experts at 5003 / 16384 32 / 44, 90 / 113.
+    // Of the 64 x 128 and the 128 x 64 tiles two share a CU: 200 rows up to 256 of them, then what the next lines say, measured with
+    // inputs in memory.  us, 64 x 128 / 128 x 64 / 128 x 128 / 192 x 128 (three stages): K 5120, N 320 at 5003 rows 41 / 42 / 51 / 62, 6144
+    // 64 / 44 / 53 / 63, 12288 96 / 79 / 95 / 67, 16384 117 / 110 / 101 / 119; K 4096, N 256 at 5003 34 / 34 / 41 / 51, 12288 59 / 60 / 47 / 55,
+    // 16384 79 / 77 / 79 / 61; K 2048, N 1024, 8 experts at 12288 89 / - / 87 / 83, 16384 113 / - / 112 / 90.
     const auto tiles = [&](int tm, int tn) {
         return (g->T / tm + (std::min(g->E, g->T) + 1) / 2) * (long)cdiv(g->N, tn);     // experts' last tiles: half full on average
     };
     const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
     const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), c128 = cost(128, 128, 1);
     const long c192 = cost(192, 128, 1);
-    const long n64 = tiles(64, 128), last = n64 % 512, c64 = n64 / 512 * 250 + (last == 0 ? 0 : last <= 256 ? 180 : 280);
-    const long best = std::min({c11, c12, c22, c24, c64, c128, c192});
+    const auto shared = [](long n, long round, long most) { return n / 512 * round + (n % 512 == 0 ? 0 : n % 512 <= 256 ? 200 : most); };
+    const long c64 = shared(tiles(64, 128), 285, 330), c64n = shared(tiles(128, 64), 340, 390) + 1;
+    const long best = std::min({c11, c12, c22, c24, c64, c64n, c128, c192});
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
     if (best == c22) return launch_narrow<2, 2>(g, stream);
     if (best == c24) return launch_narrow<2, 4>(g, stream);
     if (best == c64) return launch_rows<FWD, 64, 3, 2>(g, stream);
+    if (best == c64n) return launch_rows<FWD, 128, 3, 2, 64>(g, stream);
     return best == c128 ? launch_rows<FWD, 128, 4>(g, stream) : launch_rows<FWD, 192, 3>(g, stream);
 }
 
