@@ -347,7 +347,9 @@ def test_a_gradient_off_its_sixteen_bytes_and_a_layer_without_bias():
     assert (layer.weight.grad.cpu().double() - want).abs().max() <= 4 * 2.0 ** -24 * 16
 
 
-@pytest.mark.parametrize('T,E,K,N,listed', [(5003, 8, 72, 1024, True), (12300, 6, 40, 320, False), (16384, 3, 136, 256, True), (9001, 1, 64, 520, True)])
+@pytest.mark.parametrize('T,E,K,N,listed', [(5003, 8, 72, 1024, True), (12300, 6, 40, 320, False), (16384, 3, 136, 256, True), (9001, 1, 64, 520, True),
+                                            (6144, 6, 72, 320, True), (6100, 5, 200, 312, False), (9000, 6, 40, 192, True),
+                                            (2500, 6, 136, 256, True), (12288, 6, 40, 256, False)])
 def test_forward_products_of_many_rows(T, E, K, N, listed):
     """Row counts at which the 64-, 128- and 192-row tiles take turns."""
     g = torch.Generator().manual_seed(T)
