@@ -398,3 +398,19 @@ def test_codes_from_layernorm_to_product_on_another_stream_and_in_replayed_graph
             graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(out, want[k]) for _, out in graphs) and torch.equal(run(xs[k]), want[k])
+
+
+@pytest.mark.parametrize('N', [257, 258, 260, 263, 383])
+@pytest.mark.parametrize('M', [40, 700, 2600])
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_rows_that_begin_anywhere(M, N, dtype):
+    """Results of odd lengths and odd strides, every element in its place and nothing beside them."""
+    x, w, b = operands(M, N, 136, M + N)
+    xq, xs = fp8.quantize_rows(x.cuda())
+    wq, ws = fp8.quantize_weight(w.cuda())
+    want, mag = oracle(xq, xs, wq, ws, b)
+    for pad in (0, 1, 3, 5):
+        out = torch.full((M, N + pad), 7.0, dtype=dtype, device='cuda')
+        got = fp8.product(xq, xs, wq, ws, b.cuda(), out=out[:, :N])
+        close(got, want, mag, wq.shape[1])
+        assert (out[:, N:] == 7).all()

@@ -224,11 +224,17 @@ __device__ __forceinline__ f32x4 gelu_f32(f32x4 v) {
     return v;
 }
 
+// Rows of any length: vectors that need only their elements' alignment (the memory takes them: 2585 x 3307 x 496 16 us,
+// 30 value by value).
+typedef f32x4 f32x4_u __attribute__((aligned(4)));
+typedef bf16x4 bf16x4_u __attribute__((aligned(2)));
+typedef bf16x8 bf16x8_u __attribute__((aligned(2)));
+
 // four columns j .. j + 3 of a row of the residual (only those below N)
 __device__ __forceinline__ f32x4 load_resid(const Args& a, long row, int j) {
     f32x4 v = {0.f, 0.f, 0.f, 0.f};
     const float* p = a.resid + row * a.ldr + j;
-    if (j + 3 < a.N && (a.ldr & 3) == 0) v = *reinterpret_cast<const f32x4*>(p);
+    if (j + 3 < a.N) v = *reinterpret_cast<const f32x4_u*>(p);
     else
         for (int r = 0; r < 4; ++r)
             if (j + r < a.N) v[r] = p[r];
@@ -237,16 +243,16 @@ __device__ __forceinline__ f32x4 load_resid(const Args& a, long row, int j) {
 
 // and of the result
 __device__ __forceinline__ void store4(const Args& a, long row, int j, f32x4 v) {
-    const bool whole = j + 3 < a.N && (a.ldo & 3) == 0;
+    const bool whole = j + 3 < a.N;
     if (a.out_f32) {
         float* o = (float*)a.out + row * a.ldo + j;
-        if (whole) *reinterpret_cast<f32x4*>(o) = v;
+        if (whole) *reinterpret_cast<f32x4_u*>(o) = v;
         else
             for (int r = 0; r < 4; ++r)
                 if (j + r < a.N) o[r] = v[r];
     } else {
         bf16* o = (bf16*)a.out + row * a.ldo + j;
-        if (whole) *reinterpret_cast<bf16x4*>(o) = pack4(v[0], v[1], v[2], v[3]);
+        if (whole) *reinterpret_cast<bf16x4_u*>(o) = pack4(v[0], v[1], v[2], v[3]);
         else
             for (int r = 0; r < 4; ++r)
                 if (j + r < a.N) o[r] = (bf16)v[r];
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
         }
         return;
     }
-    if (OUT == VP_BF16 && ((a.N | (int)a.ldo) & 7) == 0) {
+    if constexpr (OUT == VP_BF16) {
         // through a patch of LDS of the wave's own, sixteen rows at a time, so that a lane stores sixteen bytes of a row
         constexpr int SEG = FN * 2;
         char* patch = lds + wave * 16 * PITCH;
@@ -447,7 +453,11 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
             for (int q = 0; q < SEG / 4; ++q) {
                 const int at = q * 64 + lane, r = at / SEG, i = iw + m * 16 + r, j = jw + at % SEG * 8;
                 const bf16x8 v = *reinterpret_cast<const bf16x8*>(patch + r * PITCH + at % SEG * 16);
-                if (i < a.M && j < a.N) *reinterpret_cast<bf16x8*>((bf16*)a.out + i * a.ldo + j) = v;
+                if (i >= a.M || j >= a.N) continue;
+                bf16* o = (bf16*)a.out + i * a.ldo + j;
+                if (j + 8 <= a.N) *reinterpret_cast<bf16x8_u*>(o) = v;
+                else
+                    for (int e = 0; e < a.N - j; ++e) o[e] = v[e];
             }
         }
         return;
