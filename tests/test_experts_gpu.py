@@ -382,3 +382,30 @@ def test_rows_are_ordered_whichever_kernel_does_it(T, E):
         key = torch.where((some >= 0) & (some < E), some, torch.full_like(some, E)).long()
         assert torch.equal(rows.cpu().long(), torch.argsort(key, stable=True))
         assert torch.equal(offsets.cpu().long(), torch.bincount(key, minlength=E + 1).cumsum(0)[:E + 1] - torch.bincount(key, minlength=E + 1)[:E + 1])
+
+
+@pytest.mark.parametrize('T,E,K,N', [(5003, 3, 264, 776), (9000, 2, 136, 520), (2600, 24, 200, 400), (700, 40, 72, 408), (6000, 1, 1024, 392)])
+def test_gradients_of_long_reductions(T, E, K, N):
+    """dx at sizes of every tile, dW and db in one and in several slices."""
+    g = torch.Generator().manual_seed(T)
+    x, dy, w = torch.randn(T, K, generator=g).bfloat16(), torch.randn(T, N, generator=g).bfloat16(), torch.randn(E, N, K, generator=g).bfloat16()
+    ids = torch.randint(-1, E, (T,), generator=g).int()
+    ids[torch.rand(T, generator=g) < 0.3] = 0
+    rows, offsets = experts.expert_rows(ids.cuda(), E)
+    dx = experts.grouped_linear_dgrad(dy.cuda(), w.cuda(), offsets, rows).cpu().double()
+    dw, db = [t.cpu().double() for t in experts.grouped_linear_wgrad(dy.cuda(), x.cuda(), offsets, rows)]
+    alone, none = experts.grouped_linear_wgrad(dy.cuda(), x.cuda(), offsets, rows, want_bias=False)
+    assert none is None and torch.equal(alone.cpu().double(), dw)
+    u = 2.0 ** -24
+    for e in range(-1, E):
+        s = ids == e
+        d, xe = dy[s].double(), x[s].double()
+        if e < 0:
+            assert not dx[s].any()
+            continue
+        want, mag = d @ w[e].double(), d.abs() @ w[e].double().abs()
+        tol = (N + 4) * u * mag
+        assert ((dx[s] - want).abs() <= tol + 2.0 ** -8 * (want.abs() + tol)).all()
+        n = int(s.sum()) + 4
+        assert ((dw[e] - d.t() @ xe).abs() <= n * u * (d.abs().t() @ xe.abs())).all()
+        assert ((db[e] - d.sum(0)).abs() <= n * u * d.abs().sum(0)).all()

@@ -675,13 +675,17 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_narrow_kernel(Args a, int 
     }
 }
 
-// out[i] = sum over the slices of dW / db, in order
-__global__ __launch_bounds__(256) void slice_sum_kernel(const float* __restrict__ part, float* __restrict__ out, long n4,
-                                                        int slices) {
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n4; i += (long)gridDim.x * 256) {
-        f32x4 v = reinterpret_cast<const f32x4*>(part)[i];
-        for (int s = 1; s < slices; ++s) v += reinterpret_cast<const f32x4*>(part)[s * n4 + i];
-        reinterpret_cast<f32x4*>(out)[i] = v;
+// dw[i], then db[i] = sum over the slices, in order (float4s; part holds the slices of dW, then those of db)
+__global__ __launch_bounds__(256) void slice_sum_kernel(const f32x4* __restrict__ part, f32x4* __restrict__ dw, long n,
+                                                        f32x4* __restrict__ db, long nb, int slices) {
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n + nb; i += (long)gridDim.x * 256) {
+        const bool bias = i >= n;
+        const f32x4* p = bias ? part + slices * n + (i - n) : part + i;
+        const long step = bias ? nb : n;
+        f32x4 v = p[0];
+        for (int s = 1; s < slices; ++s) v += p[s * step];
+        if (bias) db[i - n] = v;
+        else dw[i] = v;
     }
 }
 
@@ -908,6 +912,18 @@ int row_tiles(const vp_grouped_args* g, int bm) {
     return (int)(g->T / bm + groups + (g->zero_rest ? 1 : 0));
 }
 
+// Row tiles that there will probably be: experts' last tiles are half full on average, of many experts' a little less, and every
+// expert with a row has one.
+long likely_tiles(const vp_grouped_args* g, int bm) {
+    const long e = std::min(g->E, g->T);
+    return std::max(g->T / bm + (e + 1) / 2 + e / 8, e);
+}
+
+// Operand rows that n tiles of 64 x 128 cost a CU, two of which share one: a round of 512, the first 256, more of the last round
+long shared_cost(long n, long round, long most) {
+    return n / 512 * round + (n % 512 == 0 ? 0 : n % 512 <= 256 ? 200 : most);
+}
+
 template <int FM, int FN>
 int launch_narrow(const vp_grouped_args* g, hipStream_t stream) {
     const int tj = cdiv(g->N, 16 * FN);
@@ -976,14 +992,11 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // inputs in memory.  us, 64 x 128 / 128 x 64 / 128 x 128 / 192 x 128 (three stages): K 5120, N 320 at 5003 rows 41 / 42 / 51 / 62, 6144
     // 64 / 44 / 53 / 63, 12288 96 / 79 / 95 / 67, 16384 117 / 110 / 101 / 119; K 4096, N 256 at 5003 34 / 34 / 41 / 51, 12288 59 / 60 / 47 / 55,
     // 16384 79 / 77 / 79 / 61; K 2048, N 1024, 8 experts at 12288 89 / - / 87 / 83, 16384 113 / - / 112 / 90.
-    const auto tiles = [&](int tm, int tn) {
-        return (g->T / tm + (std::min(g->E, g->T) + 1) / 2) * (long)cdiv(g->N, tn);     // experts' last tiles: half full on average
-    };
+    const auto tiles = [&](int tm, int tn) { return likely_tiles(g, tm) * cdiv(g->N, tn); };
     const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
     const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), c128 = cost(128, 128, 1);
     const long c192 = cost(192, 128, 1);
-    const auto shared = [](long n, long round, long most) { return n / 512 * round + (n % 512 == 0 ? 0 : n % 512 <= 256 ? 200 : most); };
-    const long c64 = shared(tiles(64, 128), 285, 330), c64n = shared(tiles(128, 64), 340, 390) + 1;
+    const long c64 = shared_cost(tiles(64, 128), 285, 330), c64n = shared_cost(tiles(128, 64), 340, 390) + 1;
     const long best = std::min({c11, c12, c22, c24, c64, c64n, c128, c192});
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
@@ -1001,11 +1014,15 @@ extern "C" int vp_grouped_dgrad(const vp_grouped_args* g, hipStream_t stream) {
     VP_CHECK_ARG(g->ldy >= g->N && g->ldw >= g->K && g->ldo >= g->K && g->ldy % 8 == 0 && g->ldw % 8 == 0 && g->ldo % 8 == 0);
     VP_CHECK_ARG(g->stride_w % 8 == 0);
     // us at 192 / 1536 / 6144 / 12288 rows (skewed shares) for W of 320 x 4096, six experts: columns in a run 9.6 / 16 / 31 / 62,
-    // 64 x 128 tiles 7.8 / 17 / 44 / 81, 128 x 128 tiles 9.5 / 24 / 50 / 87; 768 x 4096: 64 x 128 16 / 29 / 93 / 176, 128 x 128
-    // 13.5 / 35 / 86 / 160; 1024 x 1024, 24 experts: 13 / 18 / 29 / 47 against 14 / 26 / 38 / 51 (128-row tiles half empty)
+    // 64 x 128 tiles 7.8 / 17 / 44 / 81, 128 x 128 tiles 9.5 / 24 / 50 / 87.  Tiles as for the forward product, but for the shortest
+    // reductions, where a tile is mostly beginning and end and small ones win: N 384 at 12288 rows 64 x 128 28, 192 x 128 31.  N 768,
+    // K 4096, six experts at 1536 / 5003 / 12288 rows: 64 x 128 32 / 76 / 176, chosen 29 / 64 / 145; one expert, N 752, K 3384 at 5003 64 / 49.
     if (g->N <= DX_KX * BK) return launch_dx(g, stream);
-    if (g->N <= 512 || g->T / g->E < 512) return launch_rows<DX, 64, 3>(g, stream);
-    return launch_rows<DX, 128, 4>(g, stream);
+    const auto tiles = [&](int tm) { return likely_tiles(g, tm) * cdiv(g->K, 128); };
+    const long c64 = g->N <= 384 ? 0 : shared_cost(tiles(64), 285, 330);
+    const long c128 = (tiles(128) + 255) / 256 * 256, c192 = (tiles(192) + 255) / 256 * 320;
+    if (c64 <= std::min(c128, c192)) return launch_rows<DX, 64, 3>(g, stream);
+    return c128 <= c192 ? launch_rows<DX, 128, 4>(g, stream) : launch_rows<DX, 192, 3>(g, stream);
 }
 
 extern "C" int vp_grouped_wgrad_slices(int T, int E, int N, int K) {
@@ -1029,10 +1046,10 @@ extern "C" int vp_grouped_wgrad(const vp_grouped_args* g, float* dw, float* db, 
     VP_CHECK_ARG(grid <= 0x7FFFFFFF);
     hipLaunchKernelGGL((grouped_kernel<DW, DW_BM, DW_BN, 3, 2>), dim3((unsigned)grid), dim3(THREADS), 0, stream, a, tj, ti);
     if (a.slices > 1) {
-        const int blocks = (int)(n / 4 < 2048L * 256 ? cdiv(n / 4, 256) : 2048);
-        hipLaunchKernelGGL(slice_sum_kernel, dim3(blocks), dim3(256), 0, stream, a.dw, dw, n / 4, a.slices);
-        if (db)
-            hipLaunchKernelGGL(slice_sum_kernel, dim3(cdiv(nb / 4, 256)), dim3(256), 0, stream, a.db, db, nb / 4, a.slices);
+        const long n4 = n / 4, nb4 = db ? nb / 4 : 0;
+        const int blocks = (int)std::min<long>((n4 + nb4 + 255) / 256, 2048);
+        hipLaunchKernelGGL(slice_sum_kernel, dim3(blocks), dim3(256), 0, stream, (const f32x4*)workspace, (f32x4*)dw, n4, (f32x4*)db, nb4,
+                           a.slices);
     }
     VP_LAUNCH_RET();
 }
