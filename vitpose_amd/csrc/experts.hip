@@ -934,11 +934,11 @@ int launch_narrow(const vp_grouped_args* g, hipStream_t stream) {
 }
 
 // Workgroups a row tile: as many column chunks as finish first, a workgroup costing its column tiles (kx K tiles and about
-// two more for the stores) and about six K tiles to begin.  Experts' last tiles are half full on average.
+// two more for the stores) and about six K tiles to begin.
 int launch_dx(const vp_grouped_args* g, hipStream_t stream) {
     constexpr int BM = 128, KX = DX_KX;
     const int tj = cdiv(g->K, 128), kx = cdiv(g->N, BK);
-    const long tiles = g->T / BM + (std::min(g->E, g->T) + 1) / 2;
+    const long tiles = likely_tiles(g, BM);
     int chunk = tj;
     long best = -1;
     for (int c = 1; c <= tj; ++c) {

@@ -187,6 +187,16 @@ def grouped_linear_wgrad(dy, x, offsets, rows=None, want_bias=True):
     return dw, db
 
 
+def _bf16(w):
+    """bf16 copy of f32 master weights."""
+    _on_device(w, 'weight')
+    if w.dtype is not _F32 or not w.is_contiguous() or w.data_ptr() % 16:
+        raise ValueError(f'weight: expected contiguous float32 on a 16-byte boundary, got {w.dtype}, strides {w.stride()}')
+    out = torch.empty(w.shape, dtype=_BF16, device=w.device)
+    _lib.launch(w.get_device(), 'vp_cast_f32_bf16', w.data_ptr(), out.data_ptr(), w.numel())
+    return out
+
+
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, offsets, rows, weight_bf16):
@@ -234,7 +244,7 @@ class ExpertLinear(nn.Module):
 
     def forward(self, x, expert):
         rows, offsets = expert_rows(expert, self.num_expert)
-        return _GroupedLinear.apply(x, self.weight, self.bias, offsets, rows, self.weight.detach().bfloat16())
+        return _GroupedLinear.apply(x, self.weight, self.bias, offsets, rows, _bf16(self.weight))
 
     def extra_repr(self):
         return f'num_expert={self.num_expert}, in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}'
