@@ -404,11 +404,13 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
 #pragma unroll
             for (int n = 0; n < FN; ++n) {
                 acc[m][n] = finish(a, acc[m][n], bias[n]);
+                if (jw + FN * 16 > a.N) {                     // (columns behind the end: padding)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if (jw + n * 16 + g * 4 + r >= a.N) acc[m][n][r] = 0.f;     // (columns behind the end: padding)
-                    most = max(most, abs_bits(acc[m][n][r]));
+                    for (int r = 0; r < 4; ++r)
+                        if (jw + n * 16 + g * 4 + r >= a.N) acc[m][n][r] = 0.f;
                 }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) most = max(most, abs_bits(acc[m][n][r]));
             }
             most = max(most, (uint32_t)__shfl_xor((int)most, 16, 64));
             most = max(most, (uint32_t)__shfl_xor((int)most, 32, 64));
