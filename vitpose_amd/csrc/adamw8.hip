@@ -19,7 +19,7 @@
 // 32-bit moments.  One workgroup per chunk of 2048 elements, eight per lane: sixteen lanes hold a block, so its two
 // maxima are four in-wave exchanges, and all of a lane's loads are in flight before the first is used.  The arithmetic is just
 // short enough to stay under the memory time (90 instructions an element; with the library's division and square root,
-// 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1017 us = 5.4 TB/s; 90 M 299 us, 375 with the norm in front.
+// 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1017 us = 5.4 TB/s; 90 M 299 us, 374 with the norm in front.
 #include "common.h"
 #include "vitpose_hip.h"
 
@@ -181,19 +181,35 @@ __global__ __launch_bounds__(1024) void sumsq_chunks_f64_kernel(const float* __r
     __shared__ double part[16];
     const int sub = threadIdx.x >> 8, lane = threadIdx.x & 255;      // four chunks at a time
     double d0 = 0.0, d1 = 0.0;
-    for (long c = (long)blockIdx.x * 4 + sub; c < nchunks; c += (long)gridDim.x * 4) {
-        const long s = start[c];
-        const int len = length[c];
-        if (len <= 0 || len > 2048 || (len & 3) || (s & 3) || s < 0 || s + len > numel) continue;
-        const int i = lane * 4;
-        f32x4 a = {0.f, 0.f, 0.f, 0.f}, b = a;
-        if (i < len) a = *reinterpret_cast<const f32x4*>(x + s + i);
-        if (i + 1024 < len) b = *reinterpret_cast<const f32x4*>(x + s + 1024 + i);
+    constexpr int DEEP = 2;                          // chunks in flight (90 M elements: one 69 us, two 64 = 5.9 TB/s, four 66)
+    const long stride = (long)gridDim.x * 4;
+    for (long c0 = (long)blockIdx.x * 4 + sub; c0 < nchunks; c0 += stride * DEEP) {
+        long st[DEEP];
+        int len[DEEP];
+        f32x4 v[DEEP][2];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            d0 += (double)a[k] * a[k];
-            d1 += (double)b[k] * b[k];
+        for (int d = 0; d < DEEP; ++d) {
+            const long c = c0 + d * stride;
+            st[d] = 0;
+            len[d] = 0;
+            if (c < nchunks) { st[d] = start[c]; len[d] = length[c]; }
         }
+        const int i = lane * 4;
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d) {
+            const bool ok = len[d] > 0 && len[d] <= 2048 && !(len[d] & 3) && !(st[d] & 3) && st[d] >= 0 && st[d] + len[d] <= numel;
+            v[d][0] = v[d][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+            if (ok && i < len[d]) v[d][0] = *reinterpret_cast<const f32x4*>(x + st[d] + i);
+            if (ok && i + 1024 < len[d]) v[d][1] = *reinterpret_cast<const f32x4*>(x + st[d] + 1024 + i);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int d = 0; d < DEEP; ++d)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                d0 += (double)v[d][0][k] * v[d][0][k];
+                d1 += (double)v[d][1][k] * v[d][1][k];
+            }
     }
     d0 += d1;
 #pragma unroll
