@@ -360,8 +360,8 @@ int vp_wgrad_grouped_kmap_bf16(const vp_group_entry* table_dev, int count, int t
  *     wgrad: dw [E][N][K] f32 = dy^T x, db [E][N] f32 (optional) = column sums of dy; zeros for an expert without rows.
  *            The rows are cut into s = vp_grouped_wgrad_slices(T, E, N, K) slices where there are few tiles; s > 1 needs a
  *            workspace of s E N (K + (db ? 1 : 0)) floats.  Partial sums are added up in a fixed order.
- *     zero_rest: fwd / dgrad write zeros into the rows that no expert takes (list entries behind offsets[E]); otherwise
- *     those rows are left as they are. */
+ *     zero_rest: fwd / dgrad write zeros into the rows that no expert takes (list entries before offsets[0] and behind
+ *     offsets[E]); otherwise those rows are left as they are, and so is, either way, a row that the list does not name. */
 typedef struct vp_grouped_args {
     int T, E, N, K;
     const int* offsets; const int* rows;

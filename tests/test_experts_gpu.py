@@ -409,3 +409,33 @@ def test_gradients_of_long_reductions(T, E, K, N):
         n = int(s.sum()) + 4
         assert ((dw[e] - d.t() @ xe).abs() <= n * u * (d.abs().t() @ xe.abs())).all()
         assert ((db[e] - d.sum(0)).abs() <= n * u * d.abs().sum(0)).all()
+
+
+@pytest.mark.parametrize('T,E,K,N', [(1, 2, 16, 8), (5, 2, 64, 16), (203, 3, 72, 40), (700, 40, 72, 408), (2500, 6, 136, 256), (5003, 3, 264, 776),
+                                     (6144, 6, 72, 320), (12300, 6, 40, 320), (9000, 100, 136, 520)])
+@pytest.mark.parametrize('listed', [True, False])
+@pytest.mark.parametrize('kind', ['some', 'all before', 'all behind'])
+def test_a_run_of_the_experts_leaves_zeros_in_every_other_row(T, E, K, N, listed, kind):
+    """Offsets of experts 2 .. E + 1 of E + 4: a new result has zeros in the rows of those before and behind, whatever its memory held."""
+    g = torch.Generator().manual_seed(T + N)
+    x, w, b, dy = [t.cuda() for t in data(T, E, K, N, T)]
+    ids = torch.randint(-1, E + 4, (T,), generator=g).int()
+    if kind != 'some':
+        ids.fill_(1 if kind == 'all before' else E + 2)
+    if not listed:
+        ids = torch.where(ids < 0, torch.full_like(ids, E + 9), ids).sort()[0].int()
+    rows, offsets = experts.expert_rows(ids.cuda(), E + 4)
+    rows, offsets = rows if listed else None, offsets[2:E + 3]
+    mine = ((ids >= 2) & (ids < E + 2)).cuda()
+
+    def poison(cols):
+        held = [torch.full((T, cols), float('nan'), dtype=torch.bfloat16, device='cuda') for _ in range(3)]
+        del held
+
+    for call, cols in ((lambda **k: experts.grouped_linear(x, w, b, offsets, rows, **k), N),
+                       (lambda **k: experts.grouped_linear_dgrad(dy, w, offsets, rows, **k), K)):
+        want = call(out=torch.zeros(T, cols, dtype=torch.bfloat16, device='cuda'))
+        assert not want[~mine].any() and (kind != 'some' or T < 100 or want[mine].any())
+        for _ in range(2):
+            poison(cols)
+            assert torch.equal(call(), want)

@@ -60,8 +60,8 @@ __device__ __forceinline__ Span span_of(const int* offsets, int e, int T) {
 }
 
 // What workgroup blockIdx.x of a launch over row tiles (bm list entries each, `per` workgroups a tile) has to do: the
-// expert whose rows its tile holds (E: rows behind the last expert, -1: nothing), the tile's first and last list entry and
-// the workgroup's number within the tile.  Every wave scans the experts' tile counts, 64 at a time.  The tiles there ARE are
+// expert whose rows its tile holds (E: rows behind the last expert or before the first, -1: nothing), the tile's first and last
+// list entry and the workgroup's number within the tile.  Every wave scans the experts' tile counts, 64 at a time.  The tiles there ARE are
 // dealt out to the XCDs in contiguous runs (the grid is an upper bound: dealing IT out would give seven XCDs more workgroups
 // than they have CUs and the eighth next to none; 240 of 275 workgroups: 46 us against 30).
 __device__ __forceinline__ int find_tile(const Args& a, int bm, int per, int lane, int& lo, int& hi, int& inner) {
@@ -75,18 +75,21 @@ __device__ __forceinline__ int find_tile(const Args& a, int bm, int per, int lan
         sum = wave_scan(n);
         total += __builtin_amdgcn_readlane(sum, 63);
     }
-    int end = a.T;
+    int begin = 0, end = a.T;                              // entries before begin and from end on are no expert's
     if (a.zero_rest) {
+        begin = a.offsets[0];
         end = a.offsets[a.E];
+        begin = begin < 0 ? 0 : (begin > a.T ? a.T : begin);
         end = end < 0 ? 0 : (end > a.T ? a.T : end);
     }
-    const int rest = (a.T - end + bm - 1) / bm, groups = (total + rest) * per;
+    const int rest = (a.T - end + bm - 1) / bm, head = (begin + bm - 1) / bm, groups = (total + rest + head) * per;
     if ((int)blockIdx.x >= groups) return -1;
     const int work = xcd_remap(blockIdx.x, groups), tile = work / per;
     inner = work - tile * per;
     if (tile >= total) {
-        lo = end + (tile - total) * bm;
-        hi = min(a.T, lo + bm);
+        const bool behind = tile - total < rest;
+        lo = behind ? end + (tile - total) * bm : (tile - total - rest) * bm;
+        hi = min(behind ? a.T : begin, lo + bm);
         return a.E;
     }
     int before = 0;
@@ -906,10 +909,11 @@ Args make_args(const vp_grouped_args* g) {
     return a;
 }
 
-// upper bound of the row tiles: every expert's last tile may be partial; rows behind the last expert add one more
+// upper bound of the row tiles: every expert's last tile may be partial; rows behind the last expert and before the first add
+// one more each
 int row_tiles(const vp_grouped_args* g, int bm) {
     const long groups = (long)g->E < g->T ? g->E : g->T;
-    return (int)(g->T / bm + groups + (g->zero_rest ? 1 : 0));
+    return (int)(g->T / bm + groups + (g->zero_rest ? 2 : 0));
 }
 
 // Row tiles that there will probably be: experts' last tiles are half full on average, of many experts' a little less, and every

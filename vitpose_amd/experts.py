@@ -140,8 +140,10 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
 
 def grouped_linear(x, weight, bias, offsets, rows=None, out=None):
     """out[t] = x[t] @ weight[e].T + bias[e] for every row t of expert e.  x bf16 [T, K], weight bf16 [E, N, K], bias f32
-    [E, N] or None; offsets / rows as `expert_rows` returns them (rows None: the rows lie in the order of their experts).
-    A new result has zeros in the rows that no expert takes; a given `out` keeps them as they are."""
+    [E, N] or None; offsets / rows as `expert_rows` returns them (rows None: the rows lie in the order of their experts), or
+    E + 1 neighbours of its offsets for a run of the experts.  A new result has zeros in the rows that no expert takes; a given
+    `out` keeps them as they are.  (A list that does not name every row needs an `out`: rows that it leaves out are not
+    written.)"""
     return _product(True, x, 'x', weight, bias, offsets, rows, out)
 
 
