@@ -387,7 +387,8 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K, ldx, ldw multiples of 8.
  *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias), sums in f32; K = Kp,
  *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16, at most 2^22), bias [N] f32 or NULL, act 0: none,
- *     1: GELU (erf); with out f32, resid [M][ldr >= N] f32 or NULL is added behind act (resid = out with ldr = ldo: in place).
+ *     1: GELU (erf; normal results within (14 + 3 |x| + 1.5 x^2) 2^-24 of themselves); with out f32, resid [M][ldr >= N] f32 or
+ *     NULL is added behind act (resid = out with ldr = ldo: in place).
  *     out_dtype VP_E4M3: out [M][ldo >= Np] becomes the codes and oscale [Np / 128][M] the scales that quantize_rows makes
  *     of the result (Np = N rounded up to 128, ldo a multiple of 16, no resid): the next product's rows.
  *   layernorm_fp8: q, scale as quantize_rows makes them of (x - mean) / sqrt(var + eps) gamma + beta (norm1 / norm2,

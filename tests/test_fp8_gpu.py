@@ -414,3 +414,31 @@ def test_rows_that_begin_anywhere(M, N, dtype):
         got = fp8.product(xq, xs, wq, ws, b.cuda(), out=out[:, :N])
         close(got, want, mag, wq.shape[1])
         assert (out[:, N:] == 7).all()
+
+
+@pytest.mark.parametrize('M', [1, 3, 300, 4100])
+@pytest.mark.parametrize('out_dtype', [torch.bfloat16, torch.float32, torch.float8_e4m3fn])
+def test_the_gelu_of_small_values_and_of_its_tail(M, out_dtype):
+    """The sums are zeros here, so a column's GELU is that of its bias: blocks of 128 of every size, zeros, and the tail below zero, each
+    within a few roundings of ITSELF.  With t = |x|, in U: t / (t + c) is off by 4, the fit by 2, its eight-term polynomial by what its
+    partial sums come to, at most 2 + 2.8 t, the exponential by 2 and by the three roundings of its argument, 1.5 t^2; two products and
+    the difference add 3: below 14 + 3 t + 1.5 t^2 (the first 4 count in full only near zero)."""
+    sizes = [0.0, 1e-25, 1e-12, 1e-5, 1e-4, 1e-3, 0.1, 1.0]
+    g = torch.Generator().manual_seed(M)
+    b = torch.cat([torch.randn(128, generator=g) * s for s in sizes] + [-torch.linspace(2, 5, 128), -torch.linspace(5, 11, 128)])
+    N, K = b.numel(), 256
+    x = torch.randn(M, K, generator=g).cuda()
+    wq, ws = fp8.quantize_weight(torch.zeros(N, K, device='cuda'))
+    want = (b.double() * torch.special.erfc(-b.double() * 0.5 ** 0.5) / 2).expand(M, N)
+    tol = (14 + 3 * b.double().abs() + 1.5 * b.double() ** 2) * U * want.abs()
+    for call in (lambda: fp8.product(*fp8.quantize_rows(x), wq, ws, b.cuda(), act='gelu', out_dtype=out_dtype),
+                 lambda: fp8.linear(x, wq, ws, b.cuda(), act='gelu', out_dtype=out_dtype)):
+        got = call()
+        if out_dtype == torch.float8_e4m3fn:
+            q, s = got
+            assert not s[0].any() and not q[:, :128].view(torch.uint8).any()
+            check_codes_within(want.reshape(M, -1, 128), tol.reshape(M, -1, 128), q, s)
+        else:
+            off = (got.cpu().double() - want).abs()
+            bound = tol + (2.0 ** -8 * (want.abs() + tol) if out_dtype == torch.bfloat16 else 0)
+            assert (off <= bound).all(), [f'{v:.3g}' for v in (off / bound.clamp(min=1e-300)).view(M, -1, 128).amax((0, 2)).tolist()]
