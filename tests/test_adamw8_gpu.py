@@ -381,3 +381,16 @@ def test_flat_optimizer_first_step_equals_the_32_bit_one():
     # both compute the update in f32, 20 roundings each, from the same numbers
     tol = 4 * EPS * before.abs() + 40 * EPS * (a.data - before).abs() + 1e-12
     assert ((a.data - b.data).abs() <= tol).all()
+
+
+def test_rows_whose_end_passes_64_bits_are_skipped():
+    """A start next to 2^63: start + length is negative there, so the buffer's end has to be compared by differences."""
+    p, g, st, chunks = make([2048, 500], 10)
+    far = 2 ** 63
+    extra = [(far - 4, 8, 1.0, 0.0, 0), (far - 2048, 2048, 1.0, 0.0, 0), (0, 4, 1.0, 0.0, far - 128), (0, 2048, 1.0, 0.0, far - 2048)]
+    wide = tuple(torch.cat([c, torch.tensor([e[i] for e in extra], dtype=c.dtype)]) for i, c in enumerate(chunks))
+    a, b = step(p, g, st, chunks, HYPER, 2), step(p, g, st, wide, HYPER, 2)
+    assert torch.equal(a[0], b[0]) and all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(a[2], b[2]))
+    only = tuple(c[-4:-2].contiguous() for c in wide)            # (those that the norm reads too)
+    c = step(p, g, st, only, HYPER, 2, max_grad_norm=1.0)
+    assert torch.equal(c[0], p)

@@ -90,9 +90,9 @@ __global__ __launch_bounds__(256) void adamw8_kernel(
     const int tid = threadIdx.x, i = tid * 8;
     const long s0 = chunk_start[blockIdx.x], q0 = chunk_state[blockIdx.x];
     const int len = chunk_len[blockIdx.x];
-    // a row of the table that does not fit the buffers is left out (uniform over the workgroup)
-    if (len <= 0 || len > 2048 || (len & 3) || (s0 & 3) || (q0 & 127) || s0 < 0 || q0 < 0 || s0 + len > numel ||
-        q0 + ((len + 127) & ~127) > state_numel)
+    // a row of the table that does not fit the buffers is left out (uniform over the workgroup; by differences, which stay in 64 bits)
+    if (len <= 0 || len > 2048 || (len & 3) || (s0 & 3) || (q0 & 127) || s0 < 0 || q0 < 0 || s0 > numel - len ||
+        q0 > state_numel - ((len + 127) & ~127))
         return;
     const bool on = i < len, two = i + 4 < len;
     const long o = s0 + (on ? i : 0), o2 = two ? o + 4 : o, q = q0 + (on ? i : 0);
@@ -197,7 +197,7 @@ __global__ __launch_bounds__(1024) void sumsq_chunks_f64_kernel(const float* __r
         const int i = lane * 4;
 #pragma unroll
         for (int d = 0; d < DEEP; ++d) {
-            const bool ok = len[d] > 0 && len[d] <= 2048 && !(len[d] & 3) && !(st[d] & 3) && st[d] >= 0 && st[d] + len[d] <= numel;
+            const bool ok = len[d] > 0 && len[d] <= 2048 && !(len[d] & 3) && !(st[d] & 3) && st[d] >= 0 && st[d] <= numel - len[d];
             v[d][0] = v[d][1] = f32x4{0.f, 0.f, 0.f, 0.f};
             if (ok && i < len[d]) v[d][0] = *reinterpret_cast<const f32x4*>(x + st[d] + i);
             if (ok && i + 1024 < len[d]) v[d][1] = *reinterpret_cast<const f32x4*>(x + st[d] + 1024 + i);
