@@ -567,9 +567,11 @@ int vp_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, co
  *   exp_avg = m_e4m3 * m_scale (rounded to nearest),  sqrt(exp_avg_sq) = r_e4m3 * r_scale (rounded to one of the two
  * neighbours, up with the probability that keeps the expected exp_avg_sq; never from non-zero to zero).  `noise` keys the
  * random numbers (a hash of the low 32 bits of the state position and the key): another one each step, the same on every
- * replica.  A block whose largest magnitude is under 2^-100 is stored as zeros; one that holds anything not finite gets a
- * NaN scale.  Table: chunk_len in 1..2048 and chunk_start multiples of 4, chunk_state multiples of 128, no two chunks
- * overlapping; a row that breaks this or leaves the buffers (numel = floats of p) is skipped.
+ * replica.  A block whose largest magnitude is under 2^-100 is stored as zeros, and exp_avg where the root is; one that holds
+ * anything not finite gets a NaN scale.  exp_avg_sq itself need not fit 32 bits: gradients of any finite size up to 2^126.
+ * eps: 0 or a normal number (0: an element without moments only decays).  Table: chunk_len in 1..2048 and chunk_start
+ * multiples of 4, chunk_state multiples of 128, no two chunks overlapping; a row that breaks this or leaves the buffers
+ * (numel = floats of p) is skipped.
  * norm_partials (npartials <= 256 doubles of vp_sumsq_chunks_f64, or NULL and 0): gradients are multiplied by grad_scale *
  * min(1, max_norm / (norm * grad_scale + 1e-6)). */
 int vp_adamw8_step(float* p, const float* g, void* m_e4m3, float* m_scale, void* r_e4m3, float* r_scale, void* p_bf16,

@@ -394,3 +394,44 @@ def test_rows_whose_end_passes_64_bits_are_skipped():
     only = tuple(c[-4:-2].contiguous() for c in wide)            # (those that the norm reads too)
     c = step(p, g, st, only, HYPER, 2, max_grad_norm=1.0)
     assert torch.equal(c[0], p)
+
+
+@pytest.mark.parametrize('size', [1e-28, 1e-25, 1e-18, 1e-12, 1e19, 1e25, 1e36])
+@pytest.mark.parametrize('eps', [1e-8, 0.0])
+def test_gradients_of_any_size(size, eps):
+    """What is kept is the ROOT of the second moment, so neither a gradient whose square leaves 32 bits nor eps = 0 makes a difference."""
+    p, g, st, chunks = make([300, 2048, 5], 13, state=False)
+    gen = torch.Generator().manual_seed(14)
+    for t in (1, 2, 3):
+        g = torch.zeros(g.numel())
+        for s, n in zip(chunks[0].tolist(), chunks[1].tolist()):
+            g[s:s + n] = (0.1 + torch.rand(n, generator=gen)) * (1 - 2 * torch.randint(0, 2, (n,), generator=gen)) * size
+        hyper = (3e-3, (0.9, 0.999), eps, t)
+        p1, half, st1 = step(p, g, st, chunks, hyper, t)
+        check(p, g, st, chunks, hyper, t, 1.0, p1, half, st1)
+        p, st = p1, tuple(x.cpu() for x in st1)
+
+
+def test_without_eps_what_has_no_gradient_only_decays():
+    hyper = (3e-3, (0.9, 0.999), 0.0, 1)
+    p, g, st, chunks = make([300, 2048], 15, state=False)
+    g.zero_()
+    g[7] = 2.0
+    p1, half, st1 = step(p, g, st, chunks, hyper, 1)
+    assert torch.isfinite(p1).all()
+    still = p.clone()
+    still[320:] *= 1 - 0.75 * 3e-3 * 0.1            # (the second tensor's rate and decay)
+    assert ((p1 - still).abs() <= 4 * EPS * p.abs())[torch.arange(p.numel()) != 7].all()
+    # a gradient whose root of the second moment is below the smallest scale while its first moment is not: no trace of either is kept
+    g.fill_(1e-29)
+    p2, _, st2 = step(p1, g, optim.new_state8(st[0].numel(), 'cpu'), chunks, hyper, 2)
+    p3, _, _ = step(p2, torch.zeros_like(g), tuple(x.cpu() for x in st2), chunks, (3e-3, (0.9, 0.999), 0.0, 2), 3)
+    assert torch.isfinite(p3).all() and ((p3 - p2).abs() <= 10 * 3e-3 + p2.abs() * 1e-2).all()
+
+
+def test_a_root_far_below_its_block_keeps_a_divisor_too():
+    p, g, st, chunks = make([128], 16, state=False)
+    g.fill_(1e-35)
+    g[0] = 1e14
+    _, _, st1 = step(p, g, st, chunks, HYPER, 1)
+    assert (st1[2].cpu().view(torch.uint8)[1:] == 1).all()

@@ -11,15 +11,18 @@
 //     simulated block in which half of the gradients shrink tenfold: the steps of the OTHER half have doubled after
 //     2500 iterations; with the rounding used here they stay within 5 %).
 //   * a non-zero sqrt(v) never rounds to zero (the smallest code is 2^-9 of a scale): the divisor of an element that is
-//     small in its block is too large, never eps.
+//     small in its block is too large, never eps.  Only a block whose largest root is under 2^-100 is stored as zeros, and its
+//     m with it: no m is left without the divisor that belongs to it.
+//   * v itself need not be a 32-bit number: the root is taken of squares scaled by a power of four (gradients of 1e-38 to 1e38).
 // The random numbers are a hash of the element's position and of a key that the caller gives for the step: the same
 // inputs give the same bits, on every replica.
 //
 // Memory-bound: 18 bytes a parameter (read 4 p + 4 g + 1 m + 1 r, written 4 p + 2 bf16 copy + 1 + 1) against 30 with
 // 32-bit moments.  One workgroup per chunk of 2048 elements, eight per lane: sixteen lanes hold a block, so its two
 // maxima are four in-wave exchanges, and all of a lane's loads are in flight before the first is used.  The arithmetic is just
-// short enough to stay under the memory time (90 instructions an element; with the library's division and square root,
-// 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1017 us = 5.4 TB/s; 90 M 299 us, 374 with the norm in front.
+// short enough to stay under the memory time (102 instructions an element, 0.5 % slower than the 90 without the scaling under the
+// root; with the library's division and square root, 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1025 us = 5.4 TB/s;
+// 90 M with the norm in front 380.
 #include "common.h"
 #include "vitpose_hip.h"
 
@@ -57,9 +60,9 @@ __device__ __forceinline__ void block_scale(uint32_t bits, float& scale, float& 
     if (bits >= 0x7F800000u) scale = __uint_as_float(0x7FC00000u);
 }
 
-// the e4m3 code of x in [0, 448], rounded to its lower or upper neighbour; u in [0, 1).  Below 2^-6 the spacing stays that of
-// the binade above, so there the neighbours are found 2^-6 further up.
-__device__ __forceinline__ uint32_t code_up_or_down(float x, float u) {
+// the e4m3 code of x in [0, 448], rounded to its lower or upper neighbour, but not to zero unless `zero`; u in [0, 1).  Below
+// 2^-6 the spacing stays that of the binade above, so there the neighbours are found 2^-6 further up.
+__device__ __forceinline__ uint32_t code_up_or_down(float x, float u, bool zero) {
     x = fminf(x, 448.f);
     const bool sub = x < 0.015625f;
     const float z = sub ? 0.015625f : 0.f;
@@ -68,15 +71,22 @@ __device__ __forceinline__ uint32_t code_up_or_down(float x, float u) {
     uint32_t code = (cut >> 20) - (sub ? 968u : 960u);               // exponent bias 127 -> 7
     if (u * (hi * hi - lo2) < x * x - lo2) ++code;
     code = code > 126u ? 126u : (code < 1u ? 1u : code);
-    return x > 0.f ? code : 0u;
+    return zero ? 0u : code;
 }
 
-// sqrt of a second moment, rounded to nearest but for one value in some four million: a Newton step on v rsq(v).  What lies
-// below the smallest normal number counts as zero (rsq does not take it).
-__device__ __forceinline__ float root(float v) {
+// sqrt(b2 r^2 + (1 - b2) g^2), the root rounded to nearest but for one value in some four million: a Newton step on v rsq(v).  Both
+// numbers are scaled by the power of two that brings the larger one to 1 (its exponent kept within what has a reciprocal), which
+// changes no bit of the result: nothing overflows or underflows that the result does not.
+__device__ __forceinline__ float new_root(float r, float g, float beta2, float omb2) {
+    const uint32_t top = __float_as_uint(fmaxf(fabsf(r), fabsf(g))) & 0x7F800000u;
+    const uint32_t e = top < 0x00800000u ? 0x00800000u : (top > 0x7E800000u ? 0x7E800000u : top);
+    const float scale = __uint_as_float(0x7F000000u - e);
+    r *= scale;
+    g *= scale;
+    const float v = beta2 * (r * r) + (omb2 * g) * g;
     const float y = v < 1.17549435e-38f ? 0.f : __builtin_amdgcn_rsqf(v);
     const float s = v * y;
-    return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s);
+    return __builtin_fmaf(__builtin_fmaf(-s, s, v), 0.5f * y, s) * __uint_as_float(e);
 }
 
 __global__ __launch_bounds__(256) void adamw8_kernel(
@@ -134,7 +144,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(
             const float mk = m2[l] * msc, rk = r2[l] * rsc;
             const float gk = gv[k >> 2][k & 3] * clip, pk = pv[k >> 2][k & 3];
             m[k] = mk + omb1 * (gk - mk);
-            r[k] = root(beta2 * (rk * rk) + (omb2 * gk) * gk);
+            r[k] = new_root(rk, gk, beta2, omb2);
             pv[k >> 2][k & 3] = pk * keep - (rate * m[k]) * __builtin_amdgcn_rcpf(r[k] * inv_bc2 + eps);
             const uint32_t mb = __float_as_uint(m[k]) & 0x7FFFFFFFu, rb = __float_as_uint(r[k]) & 0x7FFFFFFFu;
             mmax = mmax > mb ? mmax : mb;
@@ -146,12 +156,14 @@ __global__ __launch_bounds__(256) void adamw8_kernel(
     float mscale, minv, rscale, rinv;
     block_scale(mmax, mscale, minv);
     block_scale(rmax, rscale, rinv);
+    const float least = rinv > 0.f ? 0.f : __builtin_inff();      // roots above it have a code
+    if (rscale == 0.f) mscale = minv = 0.f;
     uint32_t rcode[2] = {0, 0};
     const uint32_t pos = (uint32_t)(unsigned long)q;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
         const float u = (float)(mix32((pos + k) ^ key) >> 8) * 5.9604644775390625e-8f;
-        rcode[k >> 2] |= code_up_or_down(r[k] * rinv, u) << (8 * (k & 3));
+        rcode[k >> 2] |= code_up_or_down(r[k] * rinv, u, !(r[k] > least)) << (8 * (k & 3));
     }
     uint2 mo;
     int t = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * minv, m[1] * minv, 0, false);
@@ -246,10 +258,12 @@ extern "C" int vp_adamw8_step(float* p, const float* g, void* m_e4m3, float* m_s
     VP_CHECK_ARG(p && g && m_e4m3 && m_scale && r_e4m3 && r_scale && chunk_start && chunk_len && chunk_lr_scale &&
                  chunk_wd && chunk_state);
     VP_CHECK_ARG((((uintptr_t)p | (uintptr_t)g) & 15) == 0 && (((uintptr_t)m_e4m3 | (uintptr_t)r_e4m3 | (uintptr_t)p_bf16) & 7) == 0);
+    // eps 0: the smallest normal number in its place, which no root of a live block notices (0 / 0 is no update)
+    const float least = eps > 0 ? (float)eps : 1.17549435e-38f;
     const float bc1 = (float)(1.0 - pow(beta1, (double)step)), inv_bc2 = (float)(1.0 / sqrt(1.0 - pow(beta2, (double)step)));
     hipLaunchKernelGGL(adamw8_kernel, dim3(nchunks), dim3(256), 0, stream, p, g, (uint8_t*)m_e4m3, m_scale,
                        (uint8_t*)r_e4m3, r_scale, (bf16*)p_bf16, chunk_start, chunk_len, chunk_lr_scale, chunk_wd,
                        chunk_state, numel, state_numel, (float)lr, (float)(1.0 - beta1), (float)beta2,
-                       (float)(1.0 - beta2), (float)eps, bc1, inv_bc2, norm_partials, npartials, max_norm, grad_scale, noise);
+                       (float)(1.0 - beta2), least, bc1, inv_bc2, norm_partials, npartials, max_norm, grad_scale, noise);
     VP_LAUNCH_RET();
 }
