@@ -439,3 +439,17 @@ def test_a_run_of_the_experts_leaves_zeros_in_every_other_row(T, E, K, N, listed
         for _ in range(2):
             poison(cols)
             assert torch.equal(call(), want)
+
+
+def test_a_result_in_an_operand_s_memory_is_refused():
+    T, E, N = 40, 3, 64
+    x, w, b, _ = [t.cuda() for t in data(T, E, N, N, 12)]
+    rows, offsets = experts.expert_rows(routing(T, E, 'even', 1).cuda(), E)
+    for call in (lambda out: experts.grouped_linear(x, w, b, offsets, rows, out=out), lambda out: experts.grouped_linear_dgrad(x, w, offsets, rows, out=out)):
+        for out in (x, w.view(-1, N)[:T], w.view(-1)[64:64 + T * N].view(T, N)):
+            with pytest.raises(ValueError):
+                call(out)
+    both = torch.zeros(T, 2 * N, dtype=torch.bfloat16, device='cuda')       # beside each other in one array
+    both[:, :N] = x
+    y = experts.grouped_linear(both[:, :N], w, b, offsets, rows, out=both[:, N:])
+    assert torch.equal(y, experts.grouped_linear(x, w, b, offsets, rows)) and torch.equal(both[:, :N], x)

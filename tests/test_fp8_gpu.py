@@ -442,3 +442,23 @@ def test_the_gelu_of_small_values_and_of_its_tail(M, out_dtype):
             off = (got.cpu().double() - want).abs()
             bound = tol + (2.0 ** -8 * (want.abs() + tol) if out_dtype == torch.bfloat16 else 0)
             assert (off <= bound).all(), [f'{v:.3g}' for v in (off / bound.clamp(min=1e-300)).view(M, -1, 128).amax((0, 2)).tolist()]
+
+
+def test_a_result_in_an_operand_s_memory_is_refused():
+    M, N, K = 64, 64, 64
+    x, w, b = [t.cuda() for t in operands(M, N, K, 7)]
+    wq, ws = fp8.quantize_weight(w)
+    xq, xs = fp8.quantize_rows(x)
+    for out in (x, wq.view(torch.bfloat16), xq.view(torch.bfloat16)):
+        with pytest.raises(ValueError):
+            (fp8.linear if out is x else fp8.product)(*((x,) if out is x else (xq, xs)), wq, ws, out=out)
+    flat = torch.zeros(M * N + 256, device='cuda')
+    out = flat[:M * N].view(M, N)
+    for resid in (flat[4:M * N + 4].view(M, N), flat[N:M * N + N].view(M, N), flat.as_strided((M, N), (N + 4, 1))):
+        for call in (lambda **k: fp8.product(xq, xs, wq, ws, **k), lambda **k: fp8.linear(x, wq, ws, **k)):
+            with pytest.raises(ValueError):
+                call(out=out, resid=resid)
+    both = torch.zeros(M, 2 * N, device='cuda')
+    both[:, N:] = 1.0
+    y = fp8.product(xq, xs, wq, ws, out=both[:, :N], resid=both[:, N:])
+    assert torch.equal(y, fp8.product(xq, xs, wq, ws, out_dtype=torch.float32) + 1) and (both[:, N:] == 1).all()

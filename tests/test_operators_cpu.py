@@ -248,3 +248,20 @@ def test_row_counts_beyond_32_bit_arithmetic_are_refused():
     assert L.vp_grouped_fwd(ctypes.byref(a), None) == ERR_ARG
     assert L.vp_grouped_dgrad(ctypes.byref(a), None) == ERR_ARG
     assert L.vp_grouped_wgrad(ctypes.byref(a), 64, None, None, 0, None) == ERR_ARG
+
+
+def test_which_tensors_share_memory():
+    share = _lib.shares_memory
+    flat = torch.zeros(4096)
+    a = flat[:1024].view(16, 64)
+    assert share(a, a) and share(a, a[3:5]) and share(a[:, :8], a[:, 4:12]) and share(flat, a) and share(a.view(16, 8, 8), a)
+    assert not share(a, flat[1024:2048].view(16, 64)) and not share(a[:8], a[8:]) and not share(flat[1024:], a)
+    # beside each other in the rows of one array, whichever begins first, also with single rows and other types
+    assert not share(a[:, :32], a[:, 32:]) and not share(a[:, 32:], a[:, :32]) and not share(a[:9, 40:], a[2:, 8:40])
+    assert share(a[:, :33], a[:, 32:]) and share(a[:, 32:], a[1:, :33])
+    assert not share(a[3:4, :32], a[:, 32:]) and share(a[3:4, :33], a[:, 32:]) and share(a[3:4], a[3:4]) and not share(a[3:4], a[4:5])
+    half = flat.view(torch.bfloat16)[:2048].view(16, 128)
+    assert not share(half[:, :64], a[:, 32:]) and share(half[:, :66], a[:, 32:]) and not share(half[:, 64:], a[:, :32])
+    # rows of another distance: the whole ranges count
+    assert share(a[:, :8], flat[8:2056].view(16, 128)[:, :8])
+    assert not share(a, a[:0]) and not share(a[:, :0], a)

@@ -193,5 +193,25 @@ def launch(index, entry, *args):
         raise RuntimeError(f'{entry.__name__} failed: {rc}')
 
 
+def shares_memory(a, b):
+    """Whether an element of one tensor lies in the other's memory.  Two matrices whose rows lie equally far apart may lie beside each
+    other in one array; of other layouts the whole range from the first element to the last counts."""
+    if not a.numel() or not b.numel():
+        return False
+
+    def width(t, first):
+        return (sum((n - 1) * st for n, st in zip(t.shape[first:], t.stride()[first:])) + 1) * t.element_size()
+    gap = b.data_ptr() - a.data_ptr()
+    if gap >= width(a, 0) or -gap >= width(b, 0):
+        return False
+    if a.dim() == 2 and b.dim() == 2:
+        pitches = {t.stride(0) * t.element_size() for t in (a, b) if t.shape[0] > 1}
+        if len(pitches) == 1:
+            pitch = pitches.pop()
+            gap %= pitch
+            return gap < width(a, 1) or gap + width(b, 1) > pitch
+    return True
+
+
 def exported_symbols():
     return ['vp_abi_version', 'vp_build_arch'] + list(SIGNATURES)

@@ -129,6 +129,10 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
     if fresh:
         out = src.new_empty((T, cols))
     ldo = cols if fresh else _matrix(out, 'out', cols, src.device, T)
+    if not fresh:
+        for t, name in ((src, what), (weight, 'weight'), (bias, 'bias'), (offsets, 'offsets'), (rows, 'rows')):
+            if t is not None and _lib.shares_memory(out, t):
+                raise ValueError(f'out shares memory with {name}, which is read while it is written')
     if T:
         args = GroupedArgs(T, E, N, K, offsets.data_ptr(), rows.data_ptr() if rows is not None else None,
                            p if fwd else None, ld, pw, sn, se, bias.data_ptr() if bias is not None else None, sb,
@@ -143,7 +147,7 @@ def grouped_linear(x, weight, bias, offsets, rows=None, out=None):
     [E, N] or None; offsets / rows as `expert_rows` returns them (rows None: the rows lie in the order of their experts), or
     E + 1 neighbours of its offsets for a run of the experts.  A new result has zeros in the rows that no expert takes; a given
     `out` keeps them as they are.  (A list that does not name every row needs an `out`: rows that it leaves out are not
-    written.)"""
+    written.  `out` may not lie in an operand's memory.)"""
     return _product(True, x, 'x', weight, bias, offsets, rows, out)
 
 

@@ -143,6 +143,17 @@ def _result(M, N, out, out_dtype, like):
     return out, ldo, VP_F32 if out.dtype is _F32 else VP_BF16
 
 
+def _apart(out, resid, *operands):
+    """Refuses a given result that a workgroup could write while another still reads an operand there (the residual is read by the lane
+    that writes, so it may be the result itself)."""
+    for name, t in operands:
+        if t is not None and _lib.shares_memory(out, t):
+            raise ValueError(f'out shares memory with {name}, which is read while it is written')
+    if resid is not None and _lib.shares_memory(out, resid) and (
+            resid.data_ptr() != out.data_ptr() or (resid.stride(0) != out.stride(0) and out.shape[0] > 1)):
+        raise ValueError('out shares memory with resid, but is not the same matrix')
+
+
 def _weights(wq, ws, bias, act, d, dev):
     """(leading dimension of wq, N, Kp, pointer of bias); d and dev name the rows' device."""
     try:
@@ -179,7 +190,7 @@ def _residual(resid, M, N, tag, dev):
 
 def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
     """act(xq wq^T with the blocks' scales + bias) (+ resid), bf16 or f32 [M, N]; operands as the quantizers return them.
-    resid (f32 results only) may be `out` itself.  out_dtype = torch.float8_e4m3fn: (codes, scales) of the result, as
+    resid (f32 results only) may be `out` itself; nothing else may lie in its memory.  out_dtype = torch.float8_e4m3fn: (codes, scales) of the result, as
     quantize_rows would return them, but from the sums in f32 (no out, no resid)."""
     try:
         d, p = xq.get_device(), xq.data_ptr()
@@ -209,8 +220,11 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
                            VP_E4M3, None, 0, s.data_ptr())
             _lib.launch(d, _lib.lib().vp_gemm_fp8, ctypes.byref(args))
         return q, s
+    given = out is not None
     out, ldo, tag = _result(M, N, out, out_dtype, xs)
     pr, ldr = _residual(resid, M, N, tag, xq.device) if resid is not None else (None, 0)
+    if given:
+        _apart(out, resid, ('xq', xq), ('xs', xs), ('wq', wq), ('ws', ws), ('bias', bias))
     if M and N:
         args = Fp8Args(M, N, Kp, p, ldx, xs.data_ptr(), wq.data_ptr(), ldw, ws.data_ptr(), pb, _ACTS[act], out.data_ptr(), ldo, tag,
                        pr, ldr)
@@ -228,8 +242,11 @@ def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, r
     ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, x.device)
     if (K + 127) // BLOCK * BLOCK != Kp:
         raise ValueError(f'x {tuple(x.shape)} against wq {tuple(wq.shape)}')
+    given = out is not None
     out, ldo, otag = _result(M, N, out, out_dtype, x)
     pr, ldr = _residual(resid, M, N, otag, x.device) if resid is not None else (None, 0)
+    if given:
+        _apart(out, resid, ('x', x), ('wq', wq), ('ws', ws), ('bias', bias))
     if M and N:
         L = _lib.lib()
         q = s = None
