@@ -354,7 +354,8 @@ int vp_wgrad_grouped_kmap_bf16(const vp_group_entry* table_dev, int count, int t
  *   The products take such a list, or rows = NULL: entry i of the list is then row i.  Entries outside [0, T) are left
  *     out, offsets are cut to [0, T]; no row may be listed twice.  bf16 operands, sums in f32, each result rounded once.
  *     x [T][ldx >= K], w [E][N][ldw >= K] (experts stride_w apart), dy [T][ldy >= N], bias [E][N] f32 (stride_b apart).
- *     N, K and every leading dimension multiples of 8, pointers on 16 bytes, T at most 2^30.
+ *     N, K and every leading dimension multiples of 8, pointers on 16 bytes, T at most 2^30 (VP_ERR_UNSUPPORTED where the
+ *     widest tiles still need a launch of 2^32 threads).
  *     fwd:   out [T][ldo >= N] bf16 = x w^T + bias
  *     dgrad: out [T][ldo >= K] bf16 = dy w
  *     wgrad: dw [E][N][K] f32 = dy^T x, db [E][N] f32 (optional) = column sums of dy; zeros for an expert without rows.
@@ -393,7 +394,8 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *     of the result (Np = N rounded up to 128, ldo a multiple of 16, no resid): the next product's rows.
  *   layernorm_fp8: q, scale as quantize_rows makes them of (x - mean) / sqrt(var + eps) gamma + beta (norm1 / norm2,
  *     vit.py:118-140), x [M][E] f32, E a multiple of 8, at most 2048.
- * M at most 2^29.  Array starts on 16 bytes (of scales and bias: on their own 4). */
+ * M at most 2^29 (VP_ERR_UNSUPPORTED where the largest tiles still need a launch of 2^32 threads).  Array starts on 16 bytes (of
+ * scales and bias: on their own 4). */
 typedef struct vp_fp8_args {
     int M, N, K;
     const void* xq; long ldx; const float* xs;

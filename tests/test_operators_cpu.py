@@ -265,3 +265,18 @@ def test_which_tensors_share_memory():
     # rows of another distance: the whole ranges count
     assert share(a[:, :8], flat[8:2056].view(16, 128)[:, :8])
     assert not share(a, a[:0]) and not share(a[:, :0], a)
+
+
+def test_no_kernel_is_chosen_that_needs_more_threads_than_a_launch_takes():
+    """2^32 threads: 2^23 workgroups of 512."""
+    L, unsupported = _lib.lib(), -2
+    assert L.vp_linear_fp8_fused(16, 8, 128, 1) == 1
+    for M in (1 << 28, 1 << 29):             # 16 rows a workgroup: 2^24 and more of them
+        assert L.vp_linear_fp8_fused(M, 8, 128, 1) == 0
+    big = 1 << 29
+    assert fp8_gemm(M=big, N=1024, ldo=1024) == unsupported
+    assert fp8_gemm(M=big, N=1024, ldo=1024, act=1) == unsupported
+    assert grouped('vp_grouped_fwd', T=1 << 30, N=136, ldo=136, E=2) == unsupported
+    assert grouped('vp_grouped_dgrad', T=1 << 30, K=136, ldw=136, ldo=136, E=2) == unsupported
+    assert grouped('vp_grouped_dgrad', T=1 << 30, K=136, ldw=136, N=520, ldy=520, ldo=136, E=2) == unsupported
+    assert grouped('vp_grouped_wgrad', 64, 64, None, 0, T=8, E=1 << 24) == unsupported

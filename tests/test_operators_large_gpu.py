@@ -113,3 +113,37 @@ def test_adamw8_at_the_end_of_two_billion_parameters():
         assert a.shape == b.shape
         if a.dtype == torch.float32 and a.numel() == last or a.dtype == torch.uint8:
             assert torch.equal(a, b)
+
+
+def test_8_bit_products_of_more_rows_than_small_workgroups_can_be_started_for():
+    M, N, K, last = 2 ** 27 + 77, 8, 128, 50
+    g = torch.Generator().manual_seed(1)
+    w = torch.randn(N, K, generator=g).cuda()
+    wq, ws = fp8.quantize_weight(w)
+    q, s = fp8.quantize_rows(torch.randn(last, K, generator=g).cuda())
+    xq, xs = torch.zeros(M, K, dtype=torch.uint8, device='cuda').view(torch.float8_e4m3fn), torch.zeros(1, M, device='cuda')
+    xq.view(torch.uint8)[-last:], xs[:, -last:] = q.view(torch.uint8), s
+    y = fp8.product(xq, xs, wq, ws)
+    close(y[-last:], *oracle(q, s, wq, ws, None), K)
+    assert not y[:1000].any() and not y[M // 2:M - last].any()
+    del xq, xs
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device='cuda')
+    x[-last:] = 1.0
+    y = fp8.linear(x, wq, ws)
+    assert torch.equal(y[-last:], y[-1:].expand(last, N)) and not y[:M - last].any()
+    close(y[-1:], *oracle(*fp8.quantize_rows(x[-1:].clone()), wq, ws, None), K)
+
+
+def test_expert_products_of_a_billion_rows():
+    T, N, last = 2 ** 30, 8, 70
+    x = zeros_but_the_end(T, N, last, 1)
+    w = torch.randn(2, N, N, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+    offsets = torch.tensor([0, T - last, T], dtype=torch.int32, device='cuda')
+    xd, wd = x[-last:].cpu().double(), w[1].cpu().double()
+    y = experts.grouped_linear(x, w, None, offsets)
+    near(y[-last:], xd @ wd.t(), xd.abs() @ wd.abs().t(), N)
+    assert not y[:1000].any() and not y[T // 2:T // 2 + 1000].any()
+    del y
+    dx = experts.grouped_linear_dgrad(x, w, offsets)
+    near(dx[-last:], xd @ wd, xd.abs() @ wd.abs(), N)
+    assert not dx[:1000].any() and not dx[T // 2:T // 2 + 1000].any()

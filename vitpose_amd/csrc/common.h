@@ -181,6 +181,9 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// HIP starts no launch of 2^32 threads or more
+inline bool grid_fits(long groups, int threads) { return groups >= 1 && groups * threads <= 0xFFFFFFFFl; }
+
 // Bijective XCD-aware remap of a 1-D block id: blocks b and b+8 share an XCD (its L2),
 // so give each of the 8 residue classes one contiguous chunk of the tile order.
 __device__ __forceinline__ int xcd_remap(int bid, int nblk) {

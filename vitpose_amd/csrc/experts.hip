@@ -932,7 +932,7 @@ template <int FM, int FN>
 int launch_narrow(const vp_grouped_args* g, hipStream_t stream) {
     const int tj = cdiv(g->N, 16 * FN);
     const long grid = (long)row_tiles(g, 16 * FM) * tj;
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, THREADS)) return VP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((grouped_narrow_kernel<FM, FN>), dim3((unsigned)grid), dim3(THREADS), 0, stream, make_args(g), tj);
     VP_LAUNCH_RET();
 }
@@ -947,11 +947,12 @@ int launch_dx(const vp_grouped_args* g, hipStream_t stream) {
     long best = -1;
     for (int c = 1; c <= tj; ++c) {
         const int each = cdiv(tj, c);
+        if (!grid_fits((long)row_tiles(g, BM) * cdiv(tj, each), THREADS)) continue;
         const long cost = (tiles * cdiv(tj, each) + 255) / 256 * (each * (kx + 2) + 6);
         if (best < 0 || cost < best) { best = cost; chunk = each; }
     }
     const long grid = (long)row_tiles(g, BM) * cdiv(tj, chunk);
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, THREADS)) return VP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((grouped_dx_kernel<BM, KX>), dim3((unsigned)grid), dim3(THREADS), 0, stream, make_args(g), tj, chunk);
     VP_LAUNCH_RET();
 }
@@ -960,7 +961,7 @@ template <int WHAT, int BM, int S, int PER_CU = 1, int BN = 128>
 int launch_rows(const vp_grouped_args* g, hipStream_t stream) {
     const int tj = cdiv(WHAT == FWD ? g->N : g->K, BN);
     const long grid = (long)row_tiles(g, BM) * tj;
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, THREADS)) return VP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((grouped_kernel<WHAT, BM, BN, S, PER_CU>), dim3((unsigned)grid), dim3(THREADS), 0, stream, make_args(g), tj, 0);
     VP_LAUNCH_RET();
 }
@@ -1005,12 +1006,15 @@ extern "C" int vp_grouped_fwd(const vp_grouped_args* g, hipStream_t stream) {
     // inputs in memory.  us, 64 x 128 / 128 x 64 / 128 x 128 / 192 x 128 (three stages): K 5120, N 320 at 5003 rows 41 / 42 / 51 / 62, 6144
     // 64 / 44 / 53 / 63, 12288 96 / 79 / 95 / 67, 16384 117 / 110 / 101 / 119; K 4096, N 256 at 5003 34 / 34 / 41 / 51, 12288 59 / 60 / 47 / 55,
     // 16384 79 / 77 / 79 / 61; K 2048, N 1024, 8 experts at 12288 89 / - / 87 / 83, 16384 113 / - / 112 / 90.
+    constexpr long NEVER = 1l << 62;                       // (more workgroups than a launch takes)
     const auto tiles = [&](int tm, int tn) { return likely_tiles(g, tm) * cdiv(g->N, tn); };
-    const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight; };
+    const auto never = [&](int tm, int tn) { return grid_fits((long)row_tiles(g, tm) * cdiv(g->N, tn), THREADS) ? 0 : NEVER; };
+    const auto cost = [&](int tm, int tn, int weight) { return (tiles(tm, tn) + 255) / 256 * (tm + tn) * weight + never(tm, tn); };
     const long c11 = cost(16, 16, 2), c12 = cost(16, 32, 2), c22 = cost(32, 32, 2), c24 = cost(32, 64, 2), c128 = cost(128, 128, 1);
     const long c192 = cost(192, 128, 1);
-    const long c64 = shared_cost(tiles(64, 128), 285, 330), c64n = shared_cost(tiles(128, 64), 340, 390) + 1;
+    const long c64 = shared_cost(tiles(64, 128), 285, 330) + never(64, 128), c64n = shared_cost(tiles(128, 64), 340, 390) + 1 + never(128, 64);
     const long best = std::min({c11, c12, c22, c24, c64, c64n, c128, c192});
+    if (best >= NEVER) return VP_ERR_UNSUPPORTED;
     if (best == c11) return launch_narrow<1, 1>(g, stream);
     if (best == c12) return launch_narrow<1, 2>(g, stream);
     if (best == c22) return launch_narrow<2, 2>(g, stream);
@@ -1030,10 +1034,16 @@ extern "C" int vp_grouped_dgrad(const vp_grouped_args* g, hipStream_t stream) {
     // 64 x 128 tiles 7.8 / 17 / 44 / 81, 128 x 128 tiles 9.5 / 24 / 50 / 87.  Tiles as for the forward product, but for the shortest
     // reductions, where a tile is mostly beginning and end and small ones win: N 384 at 12288 rows 64 x 128 28, 192 x 128 31.  N 768,
     // K 4096, six experts at 1536 / 5003 / 12288 rows: 64 x 128 32 / 76 / 176, chosen 29 / 64 / 145; one expert, N 752, K 3384 at 5003 64 / 49.
-    if (g->N <= DX_KX * BK) return launch_dx(g, stream);
+    if (g->N <= DX_KX * BK) {
+        const int rc = launch_dx(g, stream);
+        if (rc != VP_ERR_UNSUPPORTED) return rc;
+    }
+    constexpr long NEVER = 1l << 62;
     const auto tiles = [&](int tm) { return likely_tiles(g, tm) * cdiv(g->K, 128); };
-    const long c64 = g->N <= 384 ? 0 : shared_cost(tiles(64), 285, 330);
-    const long c128 = (tiles(128) + 255) / 256 * 256, c192 = (tiles(192) + 255) / 256 * 320;
+    const auto never = [&](int tm) { return grid_fits((long)row_tiles(g, tm) * cdiv(g->K, 128), THREADS) ? 0 : NEVER; };
+    const long c64 = (g->N <= 384 ? 0 : shared_cost(tiles(64), 285, 330)) + never(64);
+    const long c128 = (tiles(128) + 255) / 256 * 256 + never(128), c192 = (tiles(192) + 255) / 256 * 320 + never(192);
+    if (std::min({c64, c128, c192}) >= NEVER) return VP_ERR_UNSUPPORTED;
     if (c64 <= std::min(c128, c192)) return launch_rows<DX, 64, 3>(g, stream);
     return c128 <= c192 ? launch_rows<DX, 128, 4>(g, stream) : launch_rows<DX, 192, 3>(g, stream);
 }
@@ -1056,7 +1066,7 @@ extern "C" int vp_grouped_wgrad(const vp_grouped_args* g, float* dw, float* db, 
     a.dw = a.slices == 1 ? dw : (float*)workspace;
     a.db = a.slices == 1 ? db : (db ? (float*)workspace + a.slices * n : nullptr);
     const long grid = ((long)g->E * tj * a.slices + 7) / 8 * 8 * ti;
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, THREADS)) return VP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((grouped_kernel<DW, DW_BM, DW_BN, 3, 2>), dim3((unsigned)grid), dim3(THREADS), 0, stream, a, tj, ti);
     if (a.slices > 1) {
         const long n4 = n / 4, nb4 = db ? nb / 4 : 0;

@@ -662,7 +662,7 @@ extern "C" int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N,
     VP_CHECK_ARG(w && q && scale && aligned16(w) && aligned16(q));
     const int KB = cdiv(K, BLK);
     const long grid = (long)KB * cdiv(N, BLK);
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, 256)) return VP_ERR_UNSUPPORTED;
     if (dtype == VP_F32)
         hipLaunchKernelGGL(quantize_weight_kernel<float>, dim3((unsigned)grid), dim3(256), 0, stream, (const float*)w, ldw, N,
                            K, KB, (uint8_t*)q, scale);
@@ -694,7 +694,7 @@ template <typename T, int FM, int FN>
 int launch_narrow(const vp_fp8_args* g, const T* x, long ldx, int K, hipStream_t stream) {
     const int tn = cdiv(g->N, 16 * FN);
     const long grid = (long)cdiv(g->M, 16 * FM) * tn;
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, 512)) return VP_ERR_UNSUPPORTED;
     hipLaunchKernelGGL((fp8_narrow_kernel<T, FM, FN>), dim3((unsigned)grid), dim3(512), 0, stream, make_args(g), x, ldx, K, tn);
     VP_LAUNCH_RET();
 }
@@ -720,13 +720,15 @@ int launch_narrow(int shape, const vp_fp8_args* g, const T* x, long ldx, int K, 
 enum { TILE_128 = 4, TILE_256 = 5 };
 constexpr int kRows[4] = {16, 16, 32, 32}, kCols[4] = {16, 32, 32, 64};
 
+// (a shape that would need more workgroups than a launch takes: never)
 int best_narrow(int M, int N, int K, double row_weight, double further, double& us) {
     int best = 0;
+    us = HUGE_VAL;
     for (int s = 0; s < 4; ++s) {
         const long wgs = (long)cdiv(M, kRows[s]) * cdiv(N, kCols[s]);
         const double rounds = (double)((wgs + 255) / 256);
         const double t = rounds * (kRows[s] * row_weight + kCols[s]) * K * 31e-6 + (rounds - 1) * further;
-        if (s == 0 || t < us) { us = t; best = s; }
+        if (t < us && grid_fits(wgs, 512)) { us = t; best = s; }
     }
     return best;
 }
@@ -736,6 +738,7 @@ int product_kernel(int M, int N, int K, int act, bool resid, double& us) {
     const double tiles = (double)cdiv(M, 128) * cdiv(N, 128) / 256, w128 = std::max(1.25, (tiles + 2 * std::ceil(tiles / 2)) / 2);
     const long w256 = ((long)cdiv(M, 256) * cdiv(N, 256) + 255) / 256;
     double t128 = w128 * (1.7 + 0.63 * kb + 1.2 * act), t256 = w256 * (7.0 + 1.84 * kb + 5.0 * act);
+    if (!grid_fits((long)cdiv(M, 128) * cdiv(N, 128), 256)) t128 = HUGE_VAL;
     const double tile = std::min(t128, t256);
     if (us <= tile) return s;
     us = tile;
@@ -753,14 +756,14 @@ int fused_kernel(int M, int N, int K, int dtype) {
     double fused, split;
     const int s = best_narrow(M, N, K, dtype == VP_F32 ? 4.0 : 2.7, 2.0, fused);
     product_kernel(M, N, K, 0, false, split);
-    return fused <= split + 4.0 ? s : -1;
+    return fused < HUGE_VAL && fused <= split + 4.0 ? s : -1;
 }
 
 template <int BM, int BN, int WN, int RING>
 int launch_tile(const vp_fp8_args* g, hipStream_t stream) {
     const int tn = cdiv(g->N, BN);
     const long grid = (long)cdiv(g->M, BM) * tn;
-    VP_CHECK_ARG(grid <= 0x7FFFFFFF);
+    if (!grid_fits(grid, 128 * WN)) return VP_ERR_UNSUPPORTED;
     auto kernel = g->out_dtype == VP_F32 ? fp8_kernel<BM, BN, WN, RING, VP_F32> : fp8_kernel<BM, BN, WN, RING, VP_BF16>;
     if constexpr (BN == BLK)
         if (g->out_dtype == VP_E4M3) kernel = fp8_kernel<BM, BN, WN, RING, VP_E4M3>;
