@@ -280,3 +280,17 @@ def test_no_kernel_is_chosen_that_needs_more_threads_than_a_launch_takes():
     assert grouped('vp_grouped_dgrad', T=1 << 30, K=136, ldw=136, ldo=136, E=2) == unsupported
     assert grouped('vp_grouped_dgrad', T=1 << 30, K=136, ldw=136, N=520, ldy=520, ldo=136, E=2) == unsupported
     assert grouped('vp_grouped_wgrad', 64, 64, None, 0, T=8, E=1 << 24) == unsupported
+
+
+def test_the_package_imports_on_a_torch_built_without_a_gpu():
+    import os
+    import subprocess
+    import sys
+    code = ("import torch\n"
+            "for name in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, name)\n"
+            "from vitpose_amd import _lib, experts, fp8, optim\n"
+            "optim.new_state8(128, 'cpu')\n"
+            "experts.ExpertLinear(2, 16, 8)\n")
+    run = subprocess.run([sys.executable, '-c', code], cwd=os.path.join(os.path.dirname(__file__), '..'), capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr

@@ -153,7 +153,7 @@ SIGNATURES = {
 }
 
 _lib = None
-_raw_stream = torch._C._cuda_getCurrentRawStream
+_raw_stream = getattr(torch._C, '_cuda_getCurrentRawStream', None)     # (a torch built without a GPU has none, and launches nothing)
 _current_device = torch.cuda.current_device if not hasattr(torch._C, '_cuda_getDevice') else torch._C._cuda_getDevice
 
 
