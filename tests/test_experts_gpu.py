@@ -453,3 +453,19 @@ def test_a_result_in_an_operand_s_memory_is_refused():
     both[:, :N] = x
     y = experts.grouped_linear(both[:, :N], w, b, offsets, rows, out=both[:, N:])
     assert torch.equal(y, experts.grouped_linear(x, w, b, offsets, rows)) and torch.equal(both[:, :N], x)
+
+
+def test_rows_and_weights_that_require_a_gradient():
+    x, w, b, dy = [t.cuda() for t in data(16, 2, 64, 32, 13)]
+    rows, offsets = experts.expert_rows(routing(16, 2, 'even', 1).cuda(), 2)
+    want = experts.grouped_linear(x, w, b, offsets, rows)
+    for call in (lambda: experts.grouped_linear(x.clone().requires_grad_(), w, b, offsets, rows),
+                 lambda: experts.grouped_linear(x, w.clone().requires_grad_(), b, offsets, rows),
+                 lambda: experts.grouped_linear_dgrad(dy.clone().requires_grad_(), w, offsets, rows),
+                 lambda: experts.grouped_linear_wgrad(dy, x.clone().requires_grad_(), offsets, rows)):
+        with pytest.raises(RuntimeError, match='requires a gradient'):
+            call()
+    with torch.no_grad():
+        assert torch.equal(experts.grouped_linear(x.clone().requires_grad_(), w.clone().requires_grad_(), b, offsets, rows), want)
+    layer = experts.ExpertLinear(2, 64, 32, device='cuda')
+    assert layer(x, routing(16, 2, 'even', 1).cuda()).requires_grad

@@ -462,3 +462,17 @@ def test_a_result_in_an_operand_s_memory_is_refused():
     both[:, N:] = 1.0
     y = fp8.product(xq, xs, wq, ws, out=both[:, :N], resid=both[:, N:])
     assert torch.equal(y, fp8.product(xq, xs, wq, ws, out_dtype=torch.float32) + 1) and (both[:, N:] == 1).all()
+
+
+def test_rows_that_require_a_gradient():
+    x, w, _ = [t.cuda() for t in operands(8, 24, 64, 8)]
+    wq, ws = fp8.quantize_weight(torch.nn.Parameter(w))
+    want = fp8.linear(x, wq, ws)
+    x.requires_grad_()
+    for call in (fp8.quantize_rows, lambda x: fp8.linear(x, wq, ws), lambda x: fp8.linear(x.detach(), wq, ws, out_dtype=torch.float32,
+                                                                                          resid=torch.zeros(8, 24, device='cuda').requires_grad_())):
+        with pytest.raises(RuntimeError, match='requires a gradient'):
+            call(x)
+    with torch.no_grad():
+        assert torch.equal(fp8.linear(x, wq, ws), want)
+    assert torch.equal(fp8.linear(x.detach(), wq, ws), want)

@@ -294,3 +294,28 @@ def test_the_package_imports_on_a_torch_built_without_a_gpu():
             "experts.ExpertLinear(2, 16, 8)\n")
     run = subprocess.run([sys.executable, '-c', code], cwd=os.path.join(os.path.dirname(__file__), '..'), capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr
+
+
+def test_rows_that_require_a_gradient_are_refused_where_none_is_recorded():
+    """(the tensors pass as far as the check: they say that they lie on a device)"""
+    from vitpose_amd import experts, fp8
+
+    class OnDevice(torch.Tensor):
+        device = torch.device('cuda', 0)
+        is_cuda = True
+
+        def get_device(self):
+            return 0
+
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype).as_subclass(OnDevice).requires_grad_()
+    x, w = t(8, 16), t(2, 8, 16)
+    offsets, f = torch.zeros(3, dtype=torch.int32), t(16, dtype=torch.float32)
+    for call in (lambda: fp8.quantize_rows(x), lambda: fp8.linear(x, x, x), lambda: fp8.layernorm_rows(t(8, 16, dtype=torch.float32), f, f),
+                 lambda: experts.grouped_linear(x, w.detach(), None, offsets), lambda: experts.grouped_linear(x.detach(), w, None, offsets),
+                 lambda: experts.grouped_linear_dgrad(t(8, 8), w.detach(), offsets), lambda: experts.grouped_linear_wgrad(t(8, 8), x.detach(), offsets)):
+        with pytest.raises(RuntimeError, match='requires a gradient'):
+            call()
+    _lib.records_none(x.detach(), 'x', '')
+    with torch.no_grad():
+        _lib.records_none(x, 'x', '')

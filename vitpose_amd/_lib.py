@@ -193,6 +193,12 @@ def launch(index, entry, *args):
         raise RuntimeError(f'{entry.__name__} failed: {rc}')
 
 
+def records_none(t, what, instead):
+    """Refuses a tensor that autograd would have to follow through an entry point that it does not see."""
+    if t is not None and t.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f'{what} requires a gradient, but this call records none: {instead}')
+
+
 def shares_memory(a, b):
     """Whether an element of one tensor lies in the other's memory.  Two matrices whose rows lie equally far apart may lie beside each
     other in one array; of other layouts the whole range from the first element to the last counts."""

@@ -8,7 +8,8 @@ row).
     dweight, dbias = grouped_linear_wgrad(dy, x, offsets, rows)     # f32 [E, N, K], [E, N]
 
 `ExpertLinear` is the module with f32 master parameters and autograd on top of them.  Operands are bf16, sums f32.  The
-routing stays on the device; nothing here synchronises.  The functions do not record gradients, the module does.
+routing stays on the device; nothing here synchronises.  The module records gradients, the functions do not (outside no_grad they
+refuse rows and weights that require one).
 """
 import ctypes
 
@@ -20,6 +21,7 @@ from ._lib import GroupedArgs
 
 MAX_EXPERTS = 512
 _BF16, _F32, _I32 = torch.bfloat16, torch.float32, torch.int32
+_INSTEAD = 'use ExpertLinear, detach it, or call under torch.no_grad()'
 _NOT_PLAIN = (AttributeError, TypeError, ValueError, RuntimeError)
 
 
@@ -99,7 +101,7 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
         d, p, pw = src.get_device(), src.data_ptr(), weight.data_ptr()
         plain = (d >= 0 and src.dtype is _BF16 and weight.dtype is _BF16 and C == (K if fwd else N) and E and N and K and
                  not ((N | K) & 7 or (p | pw) & 15) and src.is_contiguous() and weight.is_contiguous() and
-                 weight.get_device() == d and _plain_routing(offsets, rows, E, T, d) and
+                 weight.get_device() == d and not (src.requires_grad or weight.requires_grad) and _plain_routing(offsets, rows, E, T, d) and
                  (bias is None or (bias.dtype is _F32 and bias.shape == (E, N) and bias.is_contiguous() and
                                    bias.get_device() == d and not bias.data_ptr() & 15)))
     except _NOT_PLAIN:
@@ -111,6 +113,8 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
         dev = src.device
         ld = _matrix(src, what, None, dev)
         se, sn = _weight(weight, dev)
+        _lib.records_none(src, what, _INSTEAD)
+        _lib.records_none(weight, 'weight', _INSTEAD)
         E, N, K = weight.shape
         T, C = src.shape
         if C != (K if fwd else N):
@@ -130,6 +134,7 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
         out = src.new_empty((T, cols))
     ldo = cols if fresh else _matrix(out, 'out', cols, src.device, T)
     if not fresh:
+        _lib.records_none(out, 'out', _INSTEAD)
         for t, name in ((src, what), (weight, 'weight'), (bias, 'bias'), (offsets, 'offsets'), (rows, 'rows')):
             if t is not None and _lib.shares_memory(out, t):
                 raise ValueError(f'out shares memory with {name}, which is read while it is written')
@@ -164,6 +169,7 @@ def grouped_linear_wgrad(dy, x, offsets, rows=None, want_bias=True):
         d, px, py = x.get_device(), x.data_ptr(), dy.data_ptr()
         plain = (d >= 0 and T == T2 and x.dtype is _BF16 and dy.dtype is _BF16 and N and K and E >= 1 and
                  not ((N | K) & 7 or (px | py) & 15) and x.is_contiguous() and dy.is_contiguous() and dy.get_device() == d and
+                 not (x.requires_grad or dy.requires_grad) and
                  _plain_routing(offsets, rows, E, T, d))
     except _NOT_PLAIN:
         plain = False
@@ -174,6 +180,8 @@ def grouped_linear_wgrad(dy, x, offsets, rows=None, want_bias=True):
         dev, T = x.device, x.shape[0]
         ldx = _matrix(x, 'x', None, dev)
         ldy = _matrix(dy, 'dy', None, dev, T)
+        _lib.records_none(x, 'x', _INSTEAD)
+        _lib.records_none(dy, 'dy', _INSTEAD)
         _on_device(offsets, 'offsets')
         E, N, K = offsets.numel() - 1, dy.shape[1], x.shape[1]
         if E < 1:

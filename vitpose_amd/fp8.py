@@ -12,7 +12,7 @@ or, where several products read the same rows,
 `layernorm_rows` gives the rows behind a LayerNorm in that form, and a product with out_dtype = torch.float8_e4m3fn its
 result: what lies between two products then never exists in 16 bits.
 
-Kp is K rounded up to 128.  Nothing here synchronises or records gradients.
+Kp is K rounded up to 128.  Nothing here synchronises or records gradients (rows that require one are refused outside no_grad).
 """
 import ctypes
 
@@ -25,6 +25,7 @@ BLOCK = 128
 _F8, _BF16, _F32 = torch.float8_e4m3fn, torch.bfloat16, torch.float32
 _NOT_PLAIN = (AttributeError, TypeError, ValueError, RuntimeError)
 _ACTS = {None: 0, 'gelu': 1}
+_INSTEAD = 'detach it, or call under torch.no_grad()'
 
 
 def _on_device(t, what, dev=None):
@@ -73,11 +74,13 @@ def _rows(x):
     try:
         d, p = x.get_device(), x.data_ptr()
         _, K = x.shape
-        if d >= 0 and (x.dtype is _BF16 or x.dtype is _F32) and K >= 8 and not (K & 7 or p & 15) and x.is_contiguous():
+        if (d >= 0 and (x.dtype is _BF16 or x.dtype is _F32) and K >= 8 and not (K & 7 or p & 15) and x.is_contiguous() and
+                not x.requires_grad):
             return d, p, VP_BF16 if x.dtype is _BF16 else VP_F32, K
     except _NOT_PLAIN:
         pass
     tag, ld = _real_matrix(x, 'x')
+    _lib.records_none(x, 'x', _INSTEAD)
     return x.get_device(), x.data_ptr(), tag, ld
 
 
@@ -109,6 +112,7 @@ def quantize_weight(w):
 def layernorm_rows(x, weight, bias, eps=1e-6):
     """quantize_rows of the LayerNorm of x f32 [M, E] over its rows (E a multiple of 8, at most 2048)."""
     tag, ld = _real_matrix(x, 'x')
+    _lib.records_none(x, 'x', _INSTEAD)
     M, E = x.shape
     if tag != VP_F32:
         raise TypeError('x: expected float32 (the residual stream)')
@@ -140,6 +144,7 @@ def _result(M, N, out, out_dtype, like):
     ldo = out.stride(0) if M > 1 else N
     if out.numel() and ((out.stride(1) != 1 and N > 1) or ldo < N or out.data_ptr() % 16):
         raise ValueError('out: rows must be contiguous and start on a 16-byte boundary')
+    _lib.records_none(out, 'out', _INSTEAD)
     return out, ldo, VP_F32 if out.dtype is _F32 else VP_BF16
 
 
@@ -178,6 +183,7 @@ def _weights(wq, ws, bias, act, d, dev):
 def _residual(resid, M, N, tag, dev):
     """(pointer, leading dimension) of the f32 [M, N] matrix that is added to an f32 result."""
     _on_device(resid, 'resid', dev)
+    _lib.records_none(resid, 'resid', _INSTEAD)
     if tag != VP_F32:
         raise TypeError('resid: the result has to be float32 too')
     if resid.dtype is not _F32 or tuple(resid.shape) != (M, N):
