@@ -319,3 +319,19 @@ def test_rows_that_require_a_gradient_are_refused_where_none_is_recorded():
     _lib.records_none(x.detach(), 'x', '')
     with torch.no_grad():
         _lib.records_none(x, 'x', '')
+
+
+def record_fp8(monkeypatch, E, heads, B, **cfg):
+    """Entry points and workspace of an evaluation plan on 8-bit products, recorded over host buffers (nothing runs)."""
+    from vitpose_amd import engine, plan
+    monkeypatch.setattr(plan, '_p', lambda t: None if t is None else t.data_ptr())
+    cfg = dict(img_size=(256, 192), patch_size=16, in_chans=3, embed_dim=E, depth=1, num_heads=heads, mlp_ratio=4, qkv_bias=True, ratio=1, **cfg)
+    vit, ws, recorded = engine.VitRunner(cfg, engine.ParamStore(engine.vit_param_shapes(cfg), 'cpu')), engine.Workspace('cpu'), plan.Plan()
+    vit.record_forward(recorded, ws, torch.zeros(B, 3, 256, 192), B, training=False, fp8=True)
+    return [c[0] for c in recorded.calls], ws.bufs
+
+
+def test_channels_that_the_8_bit_layernorm_cannot_take_are_refused_when_the_plan_is_recorded(monkeypatch):
+    with pytest.raises(ValueError, match='embed_dim 2112'):
+        record_fp8(monkeypatch, 2112, 33, 1)
+    assert 'vp_layernorm_fp8' in record_fp8(monkeypatch, 64, 2, 1)[0]

@@ -482,6 +482,8 @@ class VitRunner:
         and fc1 read, fc1 those that fc2 reads; attention, the patch embedding and the residual stream stay what they are in
         record_forward."""
         E, T, M, Hd = self.E, self.T, B * self.T, self.hidden
+        if E > 2048:
+            raise ValueError(f'embed_dim {E}: the LayerNorm in front of 8-bit products takes at most 2048 channels (evaluate without fp8)')
         H, W = self.img_hw
         weights = self._fp8_buffers()[0]
         kbE, kbH = (E + 127) // 128, (Hd + 127) // 128
