@@ -335,3 +335,17 @@ def test_channels_that_the_8_bit_layernorm_cannot_take_are_refused_when_the_plan
     with pytest.raises(ValueError, match='embed_dim 2112'):
         record_fp8(monkeypatch, 2112, 33, 1)
     assert 'vp_layernorm_fp8' in record_fp8(monkeypatch, 64, 2, 1)[0]
+
+
+@pytest.mark.parametrize('B,few', [(2, True), (64, False)])
+@pytest.mark.parametrize('routed', [False, True])
+def test_an_8_bit_evaluation_holds_no_buffer_that_no_launch_touches(monkeypatch, B, few, routed):
+    E, Hd, M = 128, 512, 192 * B
+    calls, bufs = record_fp8(monkeypatch, E, 4, B, **(dict(num_expert=3, part_features=32) if routed else {}))
+    assert (_lib.lib().vp_linear_fp8_fused(M, E, Hd, _lib.VP_BF16) == 1) == few
+    assert calls.count('vp_gemm_fp8') == (2 if few or routed else 3)
+    codes = not few and not routed
+    assert ('h' in bufs) == (not codes) and ('fp8_hq' in bufs) == ('fp8_hs' in bufs) == codes
+    width = Hd if few and not routed else E
+    assert bufs['fp8_q'].numel() == M * width and bufs['fp8_s'].numel() == M * width // 128
+    assert not codes or (bufs['fp8_hq'].numel() == M * Hd and bufs['fp8_hs'].numel() == M * Hd // 128)

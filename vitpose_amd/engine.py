@@ -487,10 +487,14 @@ class VitRunner:
         H, W = self.img_hw
         weights = self._fp8_buffers()[0]
         kbE, kbH = (E + 127) // 128, (Hd + 127) // 128
-        xq, xs = ws.get('fp8_q', (M * max(kbE, kbH) * 128,), torch.uint8), ws.f32('fp8_s', M * max(kbE, kbH))
-        hq, hs = ws.get('fp8_hq', (M * kbH * 128,), torch.uint8), ws.f32('fp8_hs', M * kbH)
-        # fc1 hands codes to fc2 where fc2 takes codes: few rows are rounded by fc2's own kernel instead
+        # fc1 hands codes to fc2 where fc2 takes codes: few rows are rounded by fc2's own kernel instead, the routed fc2 reads bf16
         to_codes = not self.part and not plan.L.vp_linear_fp8_fused(M, E, Hd, _lib.VP_BF16)
+        kb = kbE if to_codes or self.part else max(kbE, kbH)        # (fc2 rounds its rows over the scratch too)
+        xq, xs = ws.get('fp8_q', (M * kb * 128,), torch.uint8), ws.f32('fp8_s', M * kb)
+        if to_codes:
+            hq, hs = ws.get('fp8_hq', (M * kbH * 128,), torch.uint8), ws.f32('fp8_hs', M * kbH)
+        else:
+            hact = ws.bf16('h', M, Hd)
 
         def weight(name):
             return weights[name] + (self.w(name + '.bias') if self.has(name + '.bias') else None,)
@@ -503,7 +507,7 @@ class VitRunner:
         x, xm = ws.f32('x_a', M, E), ws.f32('x_b', M, E)
         plan.gemm(col, self.h('patch_embed.proj.weight'), x, M, E, self.Kpe, ldx=self.Kpe, ldy=self.Kpe, ldo=E,
                   epilogue=_lib.VP_EPI_RESID_F32, bias=self.w('patch_embed.proj.bias'), pos=self.pos_comb, pos_rows=T)
-        qkv, ao, hact = ws.bf16('qkv', M, 3 * E), ws.bf16('ao', M, E), ws.bf16('h', M, Hd)
+        qkv, ao = ws.bf16('qkv', M, 3 * E), ws.bf16('ao', M, E)
         for i in range(self.depth):
             b = f'blocks.{i}.'
             norm(b + 'norm1', x)
