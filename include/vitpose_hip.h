@@ -573,7 +573,7 @@ int vp_adamw_step(float* p, const float* g, float* m, float* v, void* p_bf16, co
  * anything not finite gets a NaN scale.  exp_avg_sq itself need not fit 32 bits: gradients of any finite size up to 2^126.
  * eps: 0 or a normal number (0: an element without moments only decays).  Table: chunk_len in 1..2048 and chunk_start
  * multiples of 4, chunk_state multiples of 128, no two chunks overlapping; a row that breaks this or leaves the buffers
- * (numel = floats of p) is skipped.
+ * (numel = floats of p, a multiple of 4: runs are, so the last one would leave another buffer) is skipped.
  * norm_partials (npartials <= 256 doubles of vp_sumsq_chunks_f64, or NULL and 0): gradients are multiplied by grad_scale *
  * min(1, max_norm / (norm * grad_scale + 1e-6)). */
 int vp_adamw8_step(float* p, const float* g, void* m_e4m3, float* m_scale, void* r_e4m3, float* r_scale, void* p_bf16,

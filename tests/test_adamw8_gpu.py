@@ -435,3 +435,14 @@ def test_a_root_far_below_its_block_keeps_a_divisor_too():
     g[0] = 1e14
     _, _, st1 = step(p, g, st, chunks, HYPER, 1)
     assert (st1[2].cpu().view(torch.uint8)[1:] == 1).all()
+
+
+def test_a_buffer_whose_last_run_would_leave_it_is_refused():
+    p, g, st, chunks = make([2046], 17)
+    cut = [x[:2046].cuda() for x in (p, g)]
+    assert chunks[1].tolist() == [2048]
+    with pytest.raises(ValueError, match='multiple of 4'):
+        optim.adamw8_step(*cut, on_gpu(*st), on_gpu(*chunks), lr=1e-3, step=1, noise=0)
+    cut = [x[:2048].cuda() for x in (p, g)]
+    optim.adamw8_step(*cut, on_gpu(*st), on_gpu(*chunks), lr=1e-3, step=1, noise=0)
+    assert not torch.equal(cut[0].cpu(), p[:2048])

@@ -349,3 +349,8 @@ def test_an_8_bit_evaluation_holds_no_buffer_that_no_launch_touches(monkeypatch,
     width = Hd if few and not routed else E
     assert bufs['fp8_q'].numel() == M * width and bufs['fp8_s'].numel() == M * width // 128
     assert not codes or (bufs['fp8_hq'].numel() == M * Hd and bufs['fp8_hs'].numel() == M * Hd // 128)
+
+
+def test_adamw8_takes_buffers_of_whole_fours():
+    """Runs are multiples of 4 long: the last one of such a buffer, rounded up, would be skipped in silence."""
+    assert adamw8(numel=126) == ERR_ARG and adamw8(numel=129, nchunks=0) == ERR_ARG and adamw8(numel=124, nchunks=0) == 0

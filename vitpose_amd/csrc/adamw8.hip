@@ -251,7 +251,7 @@ extern "C" int vp_adamw8_step(float* p, const float* g, void* m_e4m3, float* m_s
                               const float* chunk_wd, const long* chunk_state, int nchunks, long numel, long state_numel,
                               double lr, double beta1, double beta2, double eps, long step, const double* norm_partials,
                               int npartials, float max_norm, float grad_scale, unsigned noise, hipStream_t stream) {
-    VP_CHECK_ARG(nchunks >= 0 && step > 0 && numel >= 0 && state_numel >= 0 && state_numel % 128 == 0);
+    VP_CHECK_ARG(nchunks >= 0 && step > 0 && numel >= 0 && numel % 4 == 0 && state_numel >= 0 && state_numel % 128 == 0);
     VP_CHECK_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && (eps == 0 || (eps > 0 && (float)eps >= 1.17549435e-38f)));
     VP_CHECK_ARG(npartials >= 0 && npartials <= 256 && (npartials == 0 || (norm_partials && max_norm > 0.f)));
     if (nchunks == 0) return VP_OK;

@@ -101,7 +101,7 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
                 max_grad_norm=0.0, grad_scale=1.0):
     """One AdamW step over flat f32 buffers whose moments are held in 8 bits (torch.optim.AdamW's update).
 
-    param, grad: f32 [numel];  half: bf16 [numel] copy of the new weights, or None;  state: as `new_state8` makes it;
+    param, grad: f32 [numel], numel a multiple of 4;  half: bf16 [numel] copy of the new weights, or None;  state: as `new_state8` makes it;
     chunks: device tensors (start int64, length int32, lr_scale f32, weight_decay f32, state_start int64), one entry per
     run of at most 2048 consecutive elements of one tensor (starts and lengths multiples of 4, state starts multiples
     of 128, no overlaps; an entry that leaves the buffers is skipped);  step: number of this step, from 1;  noise: key
@@ -129,6 +129,8 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
     if not 0 <= noise < 1 << 32:
         raise ValueError('noise is a 32-bit key')
     d, n, ns, nc = param.get_device(), param.numel(), m8.numel(), start.numel()
+    if n & 3:
+        raise ValueError(f'param: {n} values; a run is a multiple of 4 long, so one that reaches the end would leave the buffer: pad it')
     if nc == 0:
         return
     L = _lib.lib()
