@@ -386,7 +386,10 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *   quantize_weight: w [N][ldw >= K] f32 or bf16 -> q [N][Kp], scale [ceil(N / 128)][Kp / 128]: one per 128 x 128 square
  *     Kp = K rounded up to 128, the padding zeros; nearest, ties to even.  A block whose largest magnitude is under
  *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K, ldx, ldw multiples of 8.
- *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias), sums in f32; K = Kp,
+ *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias).  Sums in f32, but for the eight
+ *     products at a time that the matrix instruction adds first: it aligns them to the largest of the eight and keeps 13 bits below
+ *     that one's leading bit, so each of the other seven may lose up to 2^-13 of it (5e-5 of the result's norm on activations of a
+ *     transformer; the rounding of the operands is 3e-2, that of a bf16 result 2e-3).  K = Kp,
  *     xq [M][ldx >= K], wq [N][ldw >= K] (ldx, ldw multiples of 16, at most 2^22), bias [N] f32 or NULL, act 0: none,
  *     1: GELU (erf; normal results within (14 + 3 |x| + 1.5 x^2) 2^-24 of themselves); with out f32, resid [M][ldr >= N] f32 or
  *     NULL is added behind act (resid = out with ldr = ldo: in place).

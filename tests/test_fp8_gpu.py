@@ -476,3 +476,17 @@ def test_rows_that_require_a_gradient():
     with torch.no_grad():
         assert torch.equal(fp8.linear(x, wq, ws), want)
     assert torch.equal(fp8.linear(x.detach(), wq, ws), want)
+
+
+@pytest.mark.parametrize('large,small,exact', [(256.0, 2.0 ** -9, False), (16.0, 2.0 ** -5, True)])
+def test_what_the_matrix_instruction_s_eights_may_lose(large, small, exact):
+    """A large product in each eight and seven small ones, every number exact in e4m3: the sum is within 7 x 2^-13 of the large products,
+    and exact where the small ones lie within the 13 bits below."""
+    M, N, K = 300, 40, 128
+    x, w = torch.full((M, K), small), torch.ones(N, K)
+    x[:, ::8], w[:, ::8] = large, large
+    xq, wq = x.to(torch.float8_e4m3fn).cuda(), w.to(torch.float8_e4m3fn).cuda()
+    want = 16 * (large * large + 7 * small)
+    for rows in (3, M):
+        y = fp8.product(xq[:rows], torch.ones(1, rows, device='cuda'), wq, torch.ones(1, 1, device='cuda'), out_dtype=torch.float32).cpu().double()
+        assert ((y - want).abs() <= (0 if exact else 16 * 7 * 2.0 ** -13 * large * large)).all()

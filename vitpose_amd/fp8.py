@@ -12,7 +12,8 @@ or, where several products read the same rows,
 `layernorm_rows` gives the rows behind a LayerNorm in that form, and a product with out_dtype = torch.float8_e4m3fn its
 result: what lies between two products then never exists in 16 bits.
 
-Kp is K rounded up to 128.  Nothing here synchronises or records gradients (rows that require one are refused outside no_grad).
+Kp is K rounded up to 128.  Sums are f32 but for the matrix instruction's eights: it adds eight products at a time, each of which may
+lose 2^-13 of the largest of the eight (5e-5 of a result's norm, against 3e-2 for the rounding of the operands).  Nothing here synchronises or records gradients (rows that require one are refused outside no_grad).
 """
 import ctypes
 
@@ -197,7 +198,7 @@ def _residual(resid, M, N, tag, dev):
 def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, resid=None):
     """act(xq wq^T with the blocks' scales + bias) (+ resid), bf16 or f32 [M, N]; operands as the quantizers return them.
     resid (f32 results only) may be `out` itself; nothing else may lie in its memory.  out_dtype = torch.float8_e4m3fn: (codes, scales) of the result, as
-    quantize_rows would return them, but from the sums in f32 (no out, no resid)."""
+    quantize_rows would return them, but from the sums before they are rounded to 16 bits (no out, no resid)."""
     try:
         d, p = xq.get_device(), xq.data_ptr()
         M, Kx = xq.shape
