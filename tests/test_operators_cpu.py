@@ -354,3 +354,34 @@ def test_an_8_bit_evaluation_holds_no_buffer_that_no_launch_touches(monkeypatch,
 def test_adamw8_takes_buffers_of_whole_fours():
     """Runs are multiples of 4 long: the last one of such a buffer, rounded up, would be skipped in silence."""
     assert adamw8(numel=126) == ERR_ARG and adamw8(numel=129, nchunks=0) == ERR_ARG and adamw8(numel=124, nchunks=0) == 0
+
+
+def test_sizes_beyond_32_bits_are_refused_and_not_cut():
+    """(tensors without memory that say they lie on a device: nothing is allocated, and nothing must be launched)"""
+    from vitpose_amd import experts, fp8
+
+    class OnDevice(torch.Tensor):
+        device = torch.device('cuda', 0)
+        is_cuda = True
+
+        def get_device(self):
+            return 0
+
+    def t(*shape, dtype=torch.bfloat16):
+        return torch.empty(*shape, dtype=dtype, device='meta').as_subclass(OnDevice)
+    far, f8, f32, i32 = 2 ** 32 + 8, torch.float8_e4m3fn, torch.float32, torch.int32
+    wq, ws = t(8, 128, dtype=f8), t(1, 1, dtype=f32)
+    for call in (lambda: fp8.quantize_rows(t(far, 8)), lambda: fp8.quantize_rows(t(1, far)), lambda: fp8.quantize_weight(t(far, 8)),
+                 lambda: fp8.linear(t(far, 8), wq, ws), lambda: fp8.product(t(far, 128, dtype=f8), t(1, far, dtype=f32), wq, ws),
+                 lambda: fp8.product(t(4, 128, dtype=f8), t(1, 4, dtype=f32), t(far, 128, dtype=f8), t((far + 127) // 128, 1, dtype=f32)),
+                 lambda: fp8.layernorm_rows(t(far, 8, dtype=f32), t(8, dtype=f32), t(8, dtype=f32)),
+                 lambda: experts.expert_rows(t(far, dtype=i32), 4),
+                 lambda: experts.grouped_linear(t(far, 8), t(2, 16, 8), None, t(3, dtype=i32)),
+                 lambda: experts.grouped_linear(t(4, 8), t(2, far, 8), None, t(3, dtype=i32)),
+                 lambda: experts.grouped_linear_dgrad(t(far, 16), t(2, 16, 8), t(3, dtype=i32)),
+                 lambda: experts.grouped_linear_wgrad(t(far, 16), t(far, 8), t(3, dtype=i32)),
+                 lambda: optim.adamw8_step(t(8, dtype=f32), t(8, dtype=f32), (t(128, dtype=f8), ws[0], t(128, dtype=f8), ws[0]),
+                                           (t(far, dtype=torch.int64), t(far, dtype=i32), t(far, dtype=f32), t(far, dtype=f32), t(far, dtype=torch.int64)),
+                                           lr=1e-3, step=1, noise=0)):
+        with pytest.raises(ValueError, match='below 2'):
+            call()

@@ -193,6 +193,11 @@ def launch(index, entry, *args):
         raise RuntimeError(f'{entry.__name__} failed: {rc}')
 
 
+def too_large(*sizes):
+    """ctypes would cut them to 32 bits without a word."""
+    raise ValueError(f'sizes {sizes}: below 2^31 each')
+
+
 def records_none(t, what, instead):
     """Refuses a tensor that autograd would have to follow through an entry point that it does not see."""
     if t is not None and t.requires_grad and torch.is_grad_enabled():

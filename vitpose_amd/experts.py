@@ -83,6 +83,8 @@ def expert_rows(expert, num_expert):
     if not 1 <= num_expert <= MAX_EXPERTS:
         raise ValueError(f'num_expert {num_expert}: 1 to {MAX_EXPERTS} are supported')
     T = expert.shape[0]
+    if T >> 31:
+        _lib.too_large(T)
     rows, offsets = expert.new_empty(T), expert.new_empty(num_expert + 1)
     _lib.launch(expert.get_device(), _lib.lib().vp_expert_rows, expert.data_ptr(), T, num_expert, rows.data_ptr(), offsets.data_ptr())
     return rows, offsets
@@ -128,6 +130,8 @@ def _product(fwd, src, what, weight, bias, offsets, rows, out):
             if bias.stride(1) != 1 or sb % 4 or bias.data_ptr() % 16:
                 raise ValueError('bias: contiguous rows a multiple of 4 elements apart, on 16-byte boundaries')
         d, p, pw = src.get_device(), src.data_ptr(), weight.data_ptr()
+    if (T | E | N | K) >> 31:
+        _lib.too_large(T, E, N, K)
     cols = N if fwd else K
     fresh = out is None
     if fresh:
@@ -188,6 +192,8 @@ def grouped_linear_wgrad(dy, x, offsets, rows=None, want_bias=True):
             raise ValueError('offsets: at least two values are needed')
         _routing(offsets, rows, E, T, dev)
         d, px, py = x.get_device(), x.data_ptr(), dy.data_ptr()
+    if (T | E | N | K) >> 31:
+        _lib.too_large(T, E, N, K)
     dw = x.new_empty((E, N, K), dtype=_F32)
     db = x.new_empty((E, N), dtype=_F32) if want_bias else None
     L = _lib.lib()

@@ -89,6 +89,8 @@ def quantize_rows(x):
     """x f32 or bf16 [M, K] -> (e4m3 [M, Kp], f32 scales [Kp / 128, M])."""
     d, p, tag, ld = _rows(x)
     M, K = x.shape
+    if (M | K) >> 31:
+        _lib.too_large(M, K)
     kb = (K + 127) // BLOCK
     q = x.new_empty((M, kb * BLOCK), dtype=_F8)
     scale = x.new_empty((kb, M), dtype=_F32)
@@ -103,6 +105,8 @@ def quantize_weight(w):
     N, K = w.shape
     if N < 1:
         raise ValueError('w: no rows')
+    if (N | K) >> 31:
+        _lib.too_large(N, K)
     kb = (K + BLOCK - 1) // BLOCK
     q = torch.empty(N, kb * BLOCK, dtype=_F8, device=w.device)
     scale = torch.empty((N + BLOCK - 1) // BLOCK, kb, dtype=torch.float32, device=w.device)
@@ -123,6 +127,8 @@ def layernorm_rows(x, weight, bias, eps=1e-6):
         _vector(t, what, (E,), x.device)
         if t.data_ptr() % 16:
             raise ValueError(f'{what}: must start on a 16-byte boundary')
+    if M >> 31:
+        _lib.too_large(M, E)
     kb = (E + BLOCK - 1) // BLOCK
     q = x.new_empty((M, kb * BLOCK), dtype=_F8)
     scale = x.new_empty((kb, M))
@@ -217,6 +223,8 @@ def product(xq, xs, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=N
     ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, xq.device)
     if Kx != Kp:
         raise ValueError(f'xq {tuple(xq.shape)} against wq {tuple(wq.shape)}: Kp differs')
+    if (M | N | Kp) >> 31:
+        _lib.too_large(M, N, Kp)
     if out_dtype is _F8:
         if out is not None or resid is not None:
             raise ValueError('out_dtype float8_e4m3fn takes neither out nor resid')
@@ -249,6 +257,8 @@ def linear(x, wq, ws, bias=None, act=None, out_dtype=torch.bfloat16, out=None, r
     ldw, N, Kp, pb = _weights(wq, ws, bias, act, d, x.device)
     if (K + 127) // BLOCK * BLOCK != Kp:
         raise ValueError(f'x {tuple(x.shape)} against wq {tuple(wq.shape)}')
+    if (M | N | Kp) >> 31:
+        _lib.too_large(M, N, Kp)
     given = out is not None
     out, ldo, otag = _result(M, N, out, out_dtype, x)
     pr, ldr = _residual(resid, M, N, otag, x.device) if resid is not None else (None, 0)

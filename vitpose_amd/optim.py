@@ -131,6 +131,8 @@ def adamw8_step(param, grad, state, chunks, *, lr, betas=(0.9, 0.999), eps=1e-8,
     d, n, ns, nc = param.get_device(), param.numel(), m8.numel(), start.numel()
     if n & 3:
         raise ValueError(f'param: {n} values; a run is a multiple of 4 long, so one that reaches the end would leave the buffer: pad it')
+    if nc >> 31:
+        _lib.too_large(nc)
     if nc == 0:
         return
     L = _lib.lib()
