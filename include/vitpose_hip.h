@@ -354,7 +354,7 @@ int vp_wgrad_grouped_kmap_bf16(const vp_group_entry* table_dev, int count, int t
  *   The products take such a list, or rows = NULL: entry i of the list is then row i.  Entries outside [0, T) are left
  *     out, offsets are cut to [0, T]; no row may be listed twice.  bf16 operands, sums in f32, each result rounded once.
  *     x [T][ldx >= K], w [E][N][ldw >= K] (experts stride_w apart), dy [T][ldy >= N], bias [E][N] f32 (stride_b apart).
- *     N, K and every leading dimension multiples of 8, pointers on 16 bytes, T at most 2^30 (VP_ERR_UNSUPPORTED where the
+ *     N, K and every leading dimension multiples of 8, pointers on 16 bytes, T, N and K at most 2^30 (VP_ERR_UNSUPPORTED where the
  *     widest tiles still need a launch of 2^32 threads).
  *     fwd:   out [T][ldo >= N] bf16 = x w^T + bias
  *     dgrad: out [T][ldo >= K] bf16 = dy w
@@ -385,7 +385,7 @@ int vp_grouped_wgrad_slices(int T, int E, int N, int K);   /* host-side helper: 
  *   quantize_rows:   x [M][ldx >= K] f32 or bf16 -> q [M][Kp], scale [Kp / 128][M]: one scale per row and 128 values of K
  *   quantize_weight: w [N][ldw >= K] f32 or bf16 -> q [N][Kp], scale [ceil(N / 128)][Kp / 128]: one per 128 x 128 square
  *     Kp = K rounded up to 128, the padding zeros; nearest, ties to even.  A block whose largest magnitude is under
- *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K, ldx, ldw multiples of 8.
+ *     2^-100 is stored as zeros; one that holds anything not finite gets a NaN scale.  K (at most 2^30), ldx, ldw multiples of 8.
  *   gemm: out [M][ldo >= N] (bf16 or f32) = act(sum over the blocks of K of xs ws (xq . wq) + bias).  Sums in f32, but for the eight
  *     products at a time that the matrix instruction adds first: it aligns them to the largest of the eight and keeps 13 bits below
  *     that one's leading bit, so each of the other seven may lose up to 2^-13 of it (5e-5 of the result's norm on activations of a

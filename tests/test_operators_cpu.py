@@ -385,3 +385,17 @@ def test_sizes_beyond_32_bits_are_refused_and_not_cut():
                                            lr=1e-3, step=1, noise=0)):
         with pytest.raises(ValueError, match='below 2'):
             call()
+
+
+def test_rows_longer_than_32_bit_column_numbers_are_refused():
+    """A tile's or a block's last column passes 2^31 where K nearly does."""
+    far = (1 << 31) - 8
+    for entry, more in (('vp_grouped_fwd', ()), ('vp_grouped_dgrad', ()), ('vp_grouped_wgrad', (64, 64, None, 0))):
+        for over in (dict(K=far, ldx=far, ldw=far, ldo=far), dict(N=far, ldy=far, ldo=far)):
+            assert grouped(entry, *more, T=1, E=1, **over) == ERR_ARG
+    L = _lib.lib()
+    assert L.vp_quantize_fp8_rows(64, 1, far, 1, far, 64, 64, None) == ERR_ARG
+    assert L.vp_quantize_fp8_weight(64, 1, far, 1, far, 64, 64, None) == ERR_ARG
+    wide = (1 << 30) + 128
+    assert linear_fp8(K=wide, ldw=wide, k=wide, rows=wide) == ERR_ARG
+    assert linear_fp8(K=128, ldw=(1 << 22) + 128) == ERR_ARG

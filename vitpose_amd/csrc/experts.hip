@@ -866,7 +866,7 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_rows_few_kernel(const int
     for (int i = tid; i < T; i += SORT_THREADS) rows[i] = list[i];
 }
 
-constexpr int MAX_T = 1 << 30;                         // row numbers, and a tile or a run behind them, stay in 32 bits
+constexpr int MAX_T = 1 << 30;                         // row and column numbers, and a tile or a run behind them, stay in 32 bits
 
 int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
 
@@ -890,6 +890,7 @@ namespace {
 
 int check_common(const vp_grouped_args* g) {
     VP_CHECK_ARG(g && g->T >= 0 && g->T <= MAX_T && g->E >= 1 && g->N >= 8 && g->K >= 8 && g->N % 8 == 0 && g->K % 8 == 0 && g->offsets);
+    VP_CHECK_ARG(g->N <= MAX_T && g->K <= MAX_T);
     return VP_OK;
 }
 

@@ -624,7 +624,7 @@ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 extern "C" int vp_quantize_fp8_rows(const void* x, int dtype, long ldx, int M, int K, void* q, float* scale,
                                     hipStream_t stream) {
-    VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && M >= 0 && K >= 8 && K % 8 == 0 && ldx >= K && ldx % 8 == 0);
+    VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && M >= 0 && K >= 8 && K <= 1 << 30 && K % 8 == 0 && ldx >= K && ldx % 8 == 0);
     if (M == 0) return VP_OK;
     VP_CHECK_ARG(x && q && scale && aligned16(x) && aligned16(q));
     const int KB = cdiv(K, BLK);
@@ -658,7 +658,7 @@ extern "C" int vp_layernorm_fp8(const float* x, const float* gamma, const float*
 
 extern "C" int vp_quantize_fp8_weight(const void* w, int dtype, long ldw, int N, int K, void* q, float* scale,
                                       hipStream_t stream) {
-    VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && N >= 1 && K >= 8 && K % 8 == 0 && ldw >= K && ldw % 8 == 0);
+    VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && N >= 1 && K >= 8 && K <= 1 << 30 && K % 8 == 0 && ldw >= K && ldw % 8 == 0);
     VP_CHECK_ARG(w && q && scale && aligned16(w) && aligned16(q));
     const int KB = cdiv(K, BLK);
     const long grid = (long)KB * cdiv(N, BLK);
@@ -798,7 +798,7 @@ extern "C" int vp_linear_fp8(const vp_fp8_args* g, const void* x, int dtype, lon
                              hipStream_t stream) {
     if (int rc = check_fp8(g)) return rc;
     VP_CHECK_ARG((dtype == VP_F32 || dtype == VP_BF16) && K >= 8 && K % 8 == 0 && cdiv(K, BLK) * BLK == g->K);
-    VP_CHECK_ARG(ldx >= K && ldx % 8 == 0 && g->out_dtype != VP_E4M3);
+    VP_CHECK_ARG(ldx >= K && ldx % 8 == 0 && g->out_dtype != VP_E4M3 && (g->M == 0 || g->ldw <= 1 << 22));
     if (g->M == 0) return VP_OK;
     VP_CHECK_ARG(x && aligned16(x));
     const int shape = fused_kernel(g->M, g->N, K, dtype);
