@@ -21,8 +21,8 @@
 // 32-bit moments.  One workgroup per chunk of 2048 elements, eight per lane: sixteen lanes hold a block, so its two
 // maxima are four in-wave exchanges, and all of a lane's loads are in flight before the first is used.  The arithmetic is just
 // short enough to stay under the memory time (102 instructions an element, 0.5 % slower than the 90 without the scaling under the
-// root; with the library's division and square root, 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1025 us = 5.4 TB/s;
-// 90 M with the norm in front 380.
+// root; with the library's division and square root, 126, it was 3 to 10 % slower).  Measured: 304 M parameters 1018 us = 5.4 TB/s;
+// 90 M 275, with the norm in front 377.
 #include "common.h"
 #include "vitpose_hip.h"
 
@@ -193,7 +193,8 @@ __global__ __launch_bounds__(1024) void sumsq_chunks_f64_kernel(const float* __r
     __shared__ double part[16];
     const int sub = threadIdx.x >> 8, lane = threadIdx.x & 255;      // four chunks at a time
     double d0 = 0.0, d1 = 0.0;
-    constexpr int DEEP = 2;                          // chunks in flight (90 M elements: one 69 us, two 64 = 5.9 TB/s, four 66)
+    // chunks in flight (90 M elements that no cache holds: one 65 us, two 60 = 6.0 TB/s, four 62, eight 63; 100 right behind a step's writes)
+    constexpr int DEEP = 2;
     const long stride = (long)gridDim.x * 4;
     for (long c0 = (long)blockIdx.x * 4 + sub; c0 < nchunks; c0 += stride * DEEP) {
         long st[DEEP];

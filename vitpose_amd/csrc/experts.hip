@@ -173,7 +173,7 @@ __device__ __forceinline__ void wait_vm() {
 // zeros, so that the counted waits hold.  PER_CU workgroups share a CU.
 // What bounds it is what a CU takes in, 51 KB a microsecond from memory and 60 from caches, whatever the depth and however many
 // CUs are at it: without its LDS reads and matrix instructions the loop takes 40 us instead of 41.  Measured, inputs in memory:
-// forward 12288 x 256 x 4096 46 us = 560 TFLOP/s; 6144 rows of 320 x 5120: forward 43, dW 44 us (39 MB written).
+// forward 12288 x 256 x 4096 47 us = 545 TFLOP/s; 6144 rows of 320 x 5120: forward 43, dW 44 us (39 MB written).
 template <int WHAT, int BM, int BN, int S, int PER_CU = 1>
 __global__ __launch_bounds__(THREADS, 2 * PER_CU) void grouped_kernel(Args a, int tiles_j, int tiles_i) {
     constexpr bool XK = WHAT == DW, YK = WHAT != FWD;
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(THREADS, 2 * PER_CU) void grouped_kernel(Args a, in
 // 1 us of matrix instructions).  Here a workgroup keeps its rows of dy in LDS (BM rows, all of N) and runs through a
 // chunk of columns of W without a stop: the loads of the next column tile are in flight while one is finished and stored.
 // Stores that have no row or column go to a sink, so that their number, which the counted waits rely on, is known.
-// Measured: 6144 rows, 320 -> 5120, six experts 38 us (63 MB written, 530 TFLOP/s).
+// Measured: 6144 rows, 320 -> 5120, six experts 36 us (63 MB written, 560 TFLOP/s).
 __device__ float g_sink[256];
 constexpr int DX_KX = 5;       // K tiles of dy that fit beside four stages of W
 
@@ -601,8 +601,8 @@ __global__ __launch_bounds__(THREADS, 2) void grouped_dx_kernel(Args a, int tile
 // Forward product of few rows: what counts is how soon the weights have been read, by how many CUs.  A workgroup computes
 // 16 FM rows x 16 FN columns; its eight waves take every eighth chunk of 64 reduction steps straight from memory into
 // matrix-instruction operands (nobody else in the workgroup reads the same bytes, so LDS would only add a stop), four
-// chunks in flight each, and the eight partial tiles are added up in LDS in a fixed order.  Measured: one row of K 1536, N 96 5.1 us,
-// of which a launch that does nothing takes about 2; 192 rows of K 4096, N 256 11.5 us.
+// chunks in flight each, and the eight partial tiles are added up in LDS in a fixed order.  Measured: one row of K 1536, N 96 5.4 us,
+// of which a launch that does nothing takes about 2; 192 rows of K 4096, N 256 12 us.
 template <int FM, int FN>
 __global__ __launch_bounds__(THREADS, 2) void grouped_narrow_kernel(Args a, int tiles_j) {
     constexpr int TM = 16 * FM, TN = 16 * FN, DEEP = FM + FN > 4 ? 2 : 4;

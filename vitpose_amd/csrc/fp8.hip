@@ -57,7 +57,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
 
 // ---- rows: sixteen lanes hold a block of one row, a workgroup sixteen rows of DEEP blocks ----
 // HBM-bound; all loads of a lane are on their way before the first is used, and the scales of sixteen rows lie next to each other.
-// 24576 x 5120 from bf16 67 us = 5.6 TB/s (blocks dealt out one by one 77).
+// 24576 x 5120 from bf16 60 us = 6.4 TB/s (in a loop by itself 67, blocks dealt out one by one 77).
 template <typename T, int DEEP>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(const T* __restrict__ x, long ldx, int M, int K, int KB, int groups,
                                                             long work, uint8_t* __restrict__ q, float* __restrict__ scale) {
@@ -299,13 +299,13 @@ __device__ __forceinline__ f32x4 load_bias(const Args& a, int j) {
     return b;
 }
 
-// BM x BN tile, 2 x WN waves of BM / 2 x BN / WN.  What bounds the product is what the CUs take in together -- some 11 TB/s,
-// hits in L2 or not --, so the tile decides: a K tile of 128 x 128 brings 32 KB for 4.2 MFLOP, one of 256 x 256 64 KB for
-// 16.8.  LDS is a ring of RING units: behind the K tile being multiplied and the next one, the loads of RING - 2 U more units
-// are in flight (with none, the 256 x 256 tile waits for every burst of loads: 2 us a K tile for 0.9 of matrix instructions).
+// BM x BN tile, 2 x WN waves of BM / 2 x BN / WN.  128 x 128 tiles are bound by what the CUs take in together, 12.5 TB/s: a K tile
+// brings 32 KB for 4.2 MFLOP, one of 256 x 256 64 KB for 16.8, and takes in 8 TB/s; of its 156 us (below) the loads alone take 141, the
+// loop without them 128.  LDS is a ring of RING units: behind the K tile being multiplied and the next one, the loads of RING - 2 U more
+// units are in flight (with none, the 256 x 256 tile waits for every burst of loads: 2 us a K tile for 0.9 of matrix instructions).
 // A lane's accumulators are in f32 units; a K tile's product starts from zero and is added with its block's scale (one FMA
-// a value: half of the matrix instructions' time, on another unit).  Measured: 24576 x 1280 x 5120 160 us = 2.0 PFLOP/s on 256 x 256
-// tiles, 201 on 128 x 128.
+// a value: half of the matrix instructions' time, on another unit).  Measured: 24576 x 1280 x 5120 156 us by itself, 160 behind the
+// rounding of its rows = 2.0 PFLOP/s on 256 x 256 tiles, 201 on 128 x 128.
 // OUT: what is stored (the dtype tag): one kernel each, or the registers of one epilogue are spilled in another.
 template <int BM, int BN, int WN, int RING, int OUT>
 __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
@@ -522,8 +522,8 @@ __global__ __launch_bounds__(128 * WN, 2) void fp8_kernel(Args a, int tiles_n) {
 // A workgroup computes 16 FM rows x 16 FN columns; its eight waves take every eighth block of K straight from memory into
 // matrix-instruction operands, and the eight partial tiles are added up in LDS in a fixed order.  Rows in f32 or bf16 are
 // rounded to e4m3 on the way (a block of a row lies in four lanes): the same codes and scales as the quantizer's, without
-// its launch; every workgroup of a row does it again, which few rows can afford.  Measured: one row, 1280 -> 5120 5.5 us; 192 rows of
-// codes, 1024 -> 4096 with a GELU 9.6.
+// its launch; every workgroup of a row does it again, which few rows can afford.  Measured: one row, 1280 -> 5120 5.6 us; 192 rows of
+// codes, 1024 -> 4096 with a GELU 9.5.
 template <typename T, int FM, int FN>
 __global__ __launch_bounds__(512, 2) void fp8_narrow_kernel(Args a, const T* __restrict__ x, long ldx, int K, int tiles_n) {
     constexpr int TM = 16 * FM, TN = 16 * FN;
